@@ -27,6 +27,10 @@ PROLOGUE_MAX_T = 32
 SKINNY_MAX_T = 112
 
 
+DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2   # element types of rows around the layer
+NORM_MAX_COLUMNS = 16384
+NORM_PARTIAL_ROWS = 512
+TOKEN_MAX_ROWS = 1 << 30
 PARTIAL_F32, PARTIAL_HALF = 0, 1      # b200moe_problem.partial_format
 HALF_ROW_BYTES = 15232                # bytes of one row in the half form
 
@@ -126,6 +130,7 @@ class Workspace(C.Structure):
 
 
 # name -> (restype, argtypes); every symbol include/b200moe.h declares.
+_P, _I32, _I64 = C.c_void_p, C.c_int32, C.c_int64
 _PW = (C.POINTER(Problem), C.POINTER(Workspace), C.c_void_p)
 SYMBOLS = {
     "b200moe_version": (C.c_int, ()),
@@ -136,6 +141,16 @@ SYMBOLS = {
     "b200moe_workspace_init": (C.c_int, (C.POINTER(Workspace), C.c_void_p)),
     "b200moe_forward": (C.c_int, _PW),
     "b200moe_quantize_act": (C.c_int, (C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p)),
+    "b200moe_add_rms_norm": (C.c_int, (_P, _I64, _I32, _P, _I64, _I32, _P, _I32, _I32, _I32, C.c_float, _P, _P, _P, _P, _P)),
+    "b200moe_add_rms_norm_backward": (C.c_int, (_P, _I64, _I32, _P, _I64, _P, _I64, _I32, _P, _I32, _I32, _I32, C.c_float, _P,
+                                                _P, _P, _P, _P)),
+    "b200moe_token_sort_scratch_bytes": (C.c_int, (_I32, _I32, _I32, C.POINTER(C.c_size_t))),
+    "b200moe_token_sort": (C.c_int, (_P, _I32, _I32, _I32, _I32, _I32, _I32, _P, C.c_size_t, _P, _P, _P, _P, _P)),
+    "b200moe_token_gather": (C.c_int, (_P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _P)),
+    "b200moe_token_combine": (C.c_int, (_P, _I64, _I32, _P, _I32, _I32, _I32, _I32, _P, _P, _P)),
+    "b200moe_token_combine_backward": (C.c_int, (_P, _I64, _P, _I64, _I32, _P, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P)),
+    "b200moe_route_weights": (C.c_int, (_P, _P, _I32, _I32, C.c_float, _P, _P)),
+    "b200moe_route_weights_backward": (C.c_int, (_P, _P, _P, _I32, _I32, C.c_float, _P, _P)),
     "b200moe_route": (C.c_int, _PW),
     "b200moe_route_topk": (C.c_int, (C.c_void_p, C.c_void_p, C.c_int32, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p)),
     "b200moe_topk_bits": (C.c_int, _PW),

@@ -29,6 +29,18 @@ int launch_reduce(const b200moe_problem*, const b200moe_workspace*, cudaStream_t
 int launch_gemv1(const b200moe_problem*, const b200moe_workspace*, int, cudaStream_t);
 int launch_route_gemv1(const b200moe_problem*, const b200moe_workspace*, int, cudaStream_t);
 int launch_gemv2(const b200moe_problem*, const b200moe_workspace*, int, cudaStream_t);
+int launch_add_rms_norm(const void*, long long, int, const void*, long long, int, const void*, int, int, int, float, void*,
+                        void*, void*, float*, int, cudaStream_t);
+int launch_add_rms_norm_backward(const void*, long long, int, const void*, long long, const void*, long long, int, const void*,
+                                 int, int, int, float, void*, void*, void*, float*, int, cudaStream_t);
+size_t token_sort_scratch_bytes(int, int, int);
+int launch_token_sort(const int*, int, int, int, int, int, int, int*, int*, int*, int*, int*, cudaStream_t);
+int launch_token_gather(const void*, long long, int, int, int, int, const int*, const int*, void*, cudaStream_t);
+int launch_token_combine(const void*, long long, int, const float*, int, int, int, int, const int*, void*, cudaStream_t);
+int launch_token_combine_backward(const void*, long long, const void*, long long, int, const float*, int, int, int, int,
+                                  const int*, const int*, void*, float*, cudaStream_t);
+int launch_route_weights(const float*, const int*, int, int, float, float*, cudaStream_t);
+int launch_route_weights_backward(const float*, const int*, const float*, int, int, float, float*, cudaStream_t);
 
 struct DeviceInfo {
   int checked = 0;  // 0 unknown, 1 ok, -1 unsupported
@@ -194,6 +206,157 @@ int b200moe_quantize_act(const void* x_bf16, int32_t T, void* q_out, float* scal
   int sms, rc;
   if ((rc = device_info(&sms))) return rc;
   return launch_quantize_act(x_bf16, T, q_out, scale_out, sms, static_cast<cudaStream_t>(stream));
+}
+
+// ---- around the layer -------------------------------------------------------------------------------------------------
+static bool type_ok(int32_t type) { return type >= B200MOE_DTYPE_BF16 && type <= B200MOE_DTYPE_F32; }
+static long long row_bytes(int32_t columns, int32_t type) {
+  return static_cast<long long>(columns) * (type == B200MOE_DTYPE_F32 ? 4 : 2);
+}
+static bool pitch_ok(int64_t pitch) { return pitch >= 0 && (pitch & 15) == 0; }
+static long long pitch_of(int64_t pitch, int32_t columns, int32_t type) { return pitch ? pitch : row_bytes(columns, type); }
+static bool tokens_ok(int32_t T) { return T >= 0 && T <= (1 << 24); }
+
+int b200moe_add_rms_norm(const void* x, int64_t x_pitch, int32_t x_type, const void* residual, int64_t residual_pitch,
+                         int32_t residual_type, const void* weight, int32_t weight_type, int32_t T, int32_t columns,
+                         float eps, void* stream_out, void* y_out, void* q_out, float* scale_out, void* stream) {
+  if (!tokens_ok(T) || !type_ok(x_type) || !type_ok(weight_type)) return B200MOE_EINVAL;
+  if (columns < 8 || columns > B200MOE_NORM_MAX_COLUMNS || columns % 8 || (q_out && columns % QBLOCK)) return B200MOE_EINVAL;
+  if (residual && residual_type != x_type && residual_type != B200MOE_DTYPE_F32) return B200MOE_EINVAL;
+  if (!pitch_ok(x_pitch) || !pitch_ok(residual_pitch) || !(eps >= 0.f)) return B200MOE_EINVAL;
+  if (T == 0) return B200MOE_OK;
+  if (!x || !weight || (residual && !stream_out) || (!q_out != !scale_out) || (!y_out && !q_out)) return B200MOE_EINVAL;
+  if (!aligned16(x) || !aligned16(residual) || !aligned16(weight) || !aligned16(stream_out) || !aligned16(y_out) ||
+      !aligned16(q_out))
+    return B200MOE_EINVAL;
+  int sms, rc;
+  if ((rc = device_info(&sms))) return rc;
+  return launch_add_rms_norm(x, pitch_of(x_pitch, columns, x_type), x_type, residual,
+                             pitch_of(residual_pitch, columns, residual_type), residual_type, weight, weight_type, T, columns,
+                             eps, stream_out, y_out, q_out, scale_out, sms, static_cast<cudaStream_t>(stream));
+}
+
+int b200moe_add_rms_norm_backward(const void* grad_y, int64_t grad_y_pitch, int32_t type, const void* grad_stream,
+                                  int64_t grad_stream_pitch, const void* stream_rows, int64_t stream_pitch,
+                                  int32_t stream_type, const void* weight, int32_t weight_type, int32_t T, int32_t columns,
+                                  float eps, void* grad_x, void* grad_residual, void* grad_weight, float* partial,
+                                  void* stream) {
+  if (!tokens_ok(T) || !type_ok(type) || !type_ok(weight_type)) return B200MOE_EINVAL;
+  if (columns < 8 || columns > B200MOE_NORM_MAX_COLUMNS || columns % 8) return B200MOE_EINVAL;
+  if (stream_type != type && stream_type != B200MOE_DTYPE_F32) return B200MOE_EINVAL;
+  if (!pitch_ok(grad_y_pitch) || !pitch_ok(grad_stream_pitch) || !pitch_ok(stream_pitch) || !(eps >= 0.f))
+    return B200MOE_EINVAL;
+  if (T == 0) return B200MOE_OK;
+  if (!grad_y || !stream_rows || !weight || (grad_weight && !partial) || (!grad_x && !grad_residual && !grad_weight))
+    return B200MOE_EINVAL;
+  if (!aligned16(grad_y) || !aligned16(grad_stream) || !aligned16(stream_rows) || !aligned16(weight) || !aligned16(grad_x) ||
+      !aligned16(grad_residual) || !aligned16(grad_weight) || !aligned16(partial))
+    return B200MOE_EINVAL;
+  int sms, rc;
+  if ((rc = device_info(&sms))) return rc;
+  return launch_add_rms_norm_backward(grad_y, pitch_of(grad_y_pitch, columns, type), type, grad_stream,
+                                      pitch_of(grad_stream_pitch, columns, stream_type), stream_rows,
+                                      pitch_of(stream_pitch, columns, stream_type), stream_type, weight, weight_type, T,
+                                      columns, eps, grad_x, grad_residual, grad_weight, partial, sms,
+                                      static_cast<cudaStream_t>(stream));
+}
+
+static bool selection_ok(int32_t T, int32_t K) { return tokens_ok(T) && K >= 1 && K <= TOP_K; }
+// Row pieces of 16 bytes; 0 if the row is none of whole pieces.
+static int row_pieces(int32_t columns, int32_t type) {
+  if (columns < 1 || columns > (1 << 24) || !type_ok(type)) return 0;
+  const long long bytes = row_bytes(columns, type);
+  return bytes % 16 ? 0 : static_cast<int>(bytes / 16);
+}
+
+int b200moe_token_sort_scratch_bytes(int32_t T, int32_t K, int32_t E_local, size_t* bytes) {
+  if (!bytes || !selection_ok(T, K) || E_local < 1 || E_local > E_GLOBAL) return B200MOE_EINVAL;
+  *bytes = token_sort_scratch_bytes(T, K, E_local);
+  return B200MOE_OK;
+}
+
+int b200moe_token_sort(const int32_t* topk_idx, int32_t T, int32_t K, int32_t E_local, int32_t offset, int32_t align,
+                       int32_t rows, void* scratch, size_t scratch_bytes, int32_t* counts, int32_t* offsets,
+                       int32_t* row_pairs, int32_t* scatter_map, void* stream) {
+  if (!selection_ok(T, K) || E_local < 1 || E_local > E_GLOBAL || align < 1) return B200MOE_EINVAL;
+  if (rows < 0 || rows > B200MOE_TOKEN_MAX_ROWS) return B200MOE_EINVAL;
+  if (offset < 0 || offset + E_local > E_GLOBAL) return B200MOE_EINVAL;
+  if (static_cast<long long>(T) * K + static_cast<long long>(E_local) * (align - 1) > B200MOE_TOKEN_MAX_ROWS)
+    return B200MOE_EINVAL;
+  if (!counts || !offsets || (rows > 0 && !row_pairs) || (T > 0 && (!topk_idx || !scatter_map))) return B200MOE_EINVAL;
+  if (scratch_bytes < token_sort_scratch_bytes(T, K, E_local)) return B200MOE_EWORKSPACE;
+  if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 3u)) return B200MOE_EWORKSPACE;
+  int sms, rc;
+  if ((rc = device_info(&sms))) return rc;
+  return launch_token_sort(topk_idx, T, K, E_local, offset, align, rows, static_cast<int*>(scratch), counts, offsets,
+                           row_pairs, scatter_map, static_cast<cudaStream_t>(stream));
+}
+
+int b200moe_token_gather(const void* x, int64_t x_pitch, int32_t type, int32_t T, int32_t K, int32_t columns, int32_t rows,
+                         const int32_t* row_pairs, const int32_t* scatter_map, void* out, void* stream) {
+  const int pieces = row_pieces(columns, type);
+  if (!selection_ok(T, K) || !pieces || rows < 0 || rows > B200MOE_TOKEN_MAX_ROWS ||
+      !pitch_ok(x_pitch)) return B200MOE_EINVAL;
+  if (rows == 0) return B200MOE_OK;
+  if (!row_pairs || !out || (T > 0 && (!x || !scatter_map)) || !aligned16(x) || !aligned16(out)) return B200MOE_EINVAL;
+  int sms, rc;
+  if ((rc = device_info(&sms))) return rc;
+  return launch_token_gather(x, pitch_of(x_pitch, columns, type), T, K, rows, pieces, row_pairs, scatter_map, out,
+                             static_cast<cudaStream_t>(stream));
+}
+
+int b200moe_token_combine(const void* rows_in, int64_t rows_pitch, int32_t type, const float* weights, int32_t T, int32_t K,
+                          int32_t columns, int32_t rows, const int32_t* scatter_map, void* out, void* stream) {
+  const int pieces = row_pieces(columns, type);
+  if (!selection_ok(T, K) || !pieces || rows < 0 || rows > B200MOE_TOKEN_MAX_ROWS ||
+      !pitch_ok(rows_pitch)) return B200MOE_EINVAL;
+  if (T == 0) return B200MOE_OK;
+  if (!scatter_map || !out || (rows > 0 && !rows_in) || !aligned16(rows_in) || !aligned16(out)) return B200MOE_EINVAL;
+  int sms, rc;
+  if ((rc = device_info(&sms))) return rc;
+  return launch_token_combine(rows_in, pitch_of(rows_pitch, columns, type), type, weights, T, K, rows, pieces, scatter_map,
+                              out, static_cast<cudaStream_t>(stream));
+}
+
+int b200moe_token_combine_backward(const void* grad, int64_t grad_pitch, const void* rows_in, int64_t rows_pitch,
+                                   int32_t type, const float* weights, int32_t T, int32_t K, int32_t columns, int32_t rows,
+                                   const int32_t* row_pairs, const int32_t* scatter_map, void* grad_rows,
+                                   float* grad_weights, void* stream) {
+  const int pieces = row_pieces(columns, type);
+  if (!selection_ok(T, K) || !pieces || rows < 0 || rows > B200MOE_TOKEN_MAX_ROWS ||
+      !pitch_ok(grad_pitch) || !pitch_ok(rows_pitch)) return B200MOE_EINVAL;
+  if (rows == 0) grad_rows = nullptr;   // nothing to write
+  if ((T == 0 || !grad_weights) && !grad_rows) return B200MOE_OK;
+  if ((T > 0 && (!grad || !weights || !scatter_map)) || (grad_rows && !row_pairs) ||
+      (T > 0 && grad_weights && rows > 0 && !rows_in))
+    return B200MOE_EINVAL;
+  if (!aligned16(grad) || !aligned16(rows_in) || !aligned16(grad_rows)) return B200MOE_EINVAL;
+  int sms, rc;
+  if ((rc = device_info(&sms))) return rc;
+  return launch_token_combine_backward(grad, pitch_of(grad_pitch, columns, type), rows_in,
+                                       pitch_of(rows_pitch, columns, type), type, weights, T, K, rows, pieces, row_pairs,
+                                       scatter_map, grad_rows, grad_weights, static_cast<cudaStream_t>(stream));
+}
+
+int b200moe_route_weights(const float* logits, const int32_t* topk_idx, int32_t T, int32_t K, float scale, float* weights,
+                          void* stream) {
+  if (!selection_ok(T, K)) return B200MOE_EINVAL;
+  if (T == 0) return B200MOE_OK;
+  if (!logits || !topk_idx || !weights) return B200MOE_EINVAL;
+  int sms, rc;
+  if ((rc = device_info(&sms))) return rc;
+  return launch_route_weights(logits, topk_idx, T, K, scale, weights, static_cast<cudaStream_t>(stream));
+}
+
+int b200moe_route_weights_backward(const float* logits, const int32_t* topk_idx, const float* grad_weights, int32_t T,
+                                   int32_t K, float scale, float* grad_logits, void* stream) {
+  if (!selection_ok(T, K)) return B200MOE_EINVAL;
+  if (T == 0) return B200MOE_OK;
+  if (!logits || !topk_idx || !grad_weights || !grad_logits || !aligned16(grad_logits)) return B200MOE_EINVAL;
+  int sms, rc;
+  if ((rc = device_info(&sms))) return rc;
+  return launch_route_weights_backward(logits, topk_idx, grad_weights, T, K, scale, grad_logits,
+                                       static_cast<cudaStream_t>(stream));
 }
 
 int b200moe_route(const b200moe_problem* p, const b200moe_workspace* ws, void* stream) {

@@ -380,6 +380,11 @@ __host__ __device__ constexpr uint32_t umma_idesc_e4m3(int m, int n) {
 // ---------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float bf16_bits_to_float(uint16_t b) { return __uint_as_float(static_cast<uint32_t>(b) << 16); }
 
+// Two e4m3 bytes (the lower one is a's): e4m3_rn_satfinite(value * inv).
+__device__ __forceinline__ uint32_t quantize_pair(float a, float b, float inv) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(a, inv), __fmul_rn(b, inv)), __NV_SATFINITE, __NV_E4M3);
+}
+
 // Programmatic dependent launch: every kernel of the layer lets its successor be scheduled early
 // (pdl_launch_dependents at entry) and blocks in pdl_wait until its predecessor has completed and flushed before it
 // touches global memory.  Only launch latency and per-CTA set-up overlap; data dependences stay kernel-to-kernel.

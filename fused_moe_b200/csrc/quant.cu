@@ -13,10 +13,6 @@
 
 namespace b200moe {
 
-__device__ __forceinline__ uint32_t quantize_pair(float a, float b, float inv) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(a, inv), __fmul_rn(b, inv)), __NV_SATFINITE, __NV_E4M3);
-}
-
 __global__ void __launch_bounds__(256)
 k_quantize_act(const uint4* x, int T, uint2* q, float* scale) {
   const int lane = threadIdx.x & 31;

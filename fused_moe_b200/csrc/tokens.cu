@@ -1,0 +1,422 @@
+// Tokens sorted by expert and back, with weights applied, and the gradients; weights of the selected experts and theirs.
+//
+// A pair p = t * K + k is token t's k-th selected expert.  Its row is offset[e] + (pairs of expert e before p in flat order): a
+// stable counting sort, whose segments start at multiples of `align`.  Pairs of other shards' experts, negative ids, and pairs
+// whose row would lie at or behind the capacity `rows` have none (-1).  Unlike the layer's own sort (sort.cu), a token may name
+// an expert twice.
+//   gather    out[row(t,k)] = x[t]                    backward: grad_x[t] = sum_k grad[row(t,k)]    (= combine, weights 1)
+//   combine   out[t] = sum_k w[t,k] * in[row(t,k)]    backward: grad_in[row(t,k)] = w[t,k] * grad[t]
+//                                                               grad_w[t,k] = sum over columns of grad[t] * in[row(t,k)]
+// Rows without a pair are written as zeros.  The kernels walk tokens, not rows: a token's row is read once and written to (or
+// summed from) its at most eight rows.  No atomics on values, every sum in a fixed order; sums are float32.
+#include "route_token.cuh"
+#include "row_vec.cuh"
+
+namespace b200moe {
+
+constexpr int SORT_THREADS = 1024;   // pairs ranked at once by a CTA
+constexpr int SORT_WARPS = SORT_THREADS / 32;
+constexpr int SORT_MAX_CTAS = B200MOE_TOKEN_SORT_MAX_CTAS;
+
+// Index of the pair's local expert, or -1.  Unsigned: a negative id is a large one.
+__device__ __forceinline__ int local_expert(const int* topk_idx, long long p, long long n_pairs, int offset, int E_local) {
+  if (p >= n_pairs) return -1;
+  const uint32_t e = static_cast<uint32_t>(ld_dep(topk_idx + p)) - static_cast<uint32_t>(offset);
+  return e < static_cast<uint32_t>(E_local) ? static_cast<int>(e) : -1;
+}
+
+// hist[b][e] = pairs of local expert e among the `per` pairs of CTA b.
+__global__ void __launch_bounds__(SORT_THREADS)
+k_token_count(const int* topk_idx, long long n_pairs, long long per, int offset, int E_local, int* hist) {
+  __shared__ int s_count[E_GLOBAL];
+  pdl_launch_dependents();
+  if (threadIdx.x < E_GLOBAL) s_count[threadIdx.x] = 0;
+  pdl_wait();
+  __syncthreads();
+  const long long first = blockIdx.x * per;
+  for (long long i = threadIdx.x; i < per; i += SORT_THREADS) {
+    const int e = local_expert(topk_idx, first + i, n_pairs, offset, E_local);
+    if (e >= 0) atomicAdd(&s_count[e], 1);
+  }
+  __syncthreads();
+  if (threadIdx.x < E_local) hist[blockIdx.x * E_local + threadIdx.x] = s_count[threadIdx.x];
+}
+
+// The rows: every CTA derives the layout from the counts of all CTAs, then ranks its pairs SORT_THREADS at a time.  Inside a
+// warp the rank is the number of lower lanes with the same expert, and the warps' counts are prefixed per expert.
+__global__ void __launch_bounds__(SORT_THREADS)
+k_token_place(const int* topk_idx, long long n_pairs, long long per, int offset, int E_local, int align, int rows,
+              const int* hist, int* counts, int* offsets, int* row_pairs, int* scatter_map) {
+  __shared__ int s_next[E_GLOBAL];                  // row of the next pair of this expert in this CTA
+  __shared__ int s_begin[E_GLOBAL + 1];             // first row of each segment (may exceed `rows`)
+  __shared__ int s_total[E_GLOBAL];
+  __shared__ int s_scan[E_GLOBAL / 32];
+  __shared__ uint16_t s_warp[SORT_WARPS][E_GLOBAL];   // pairs of the warp, then of the warps before it
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_launch_dependents();
+  pdl_wait();
+  int total = 0, before = 0;
+  if (threadIdx.x < E_local) {
+    for (int b = 0; b < static_cast<int>(gridDim.x); ++b) {
+      if (b == static_cast<int>(blockIdx.x)) before = total;
+      total += ld_dep(hist + b * E_local + threadIdx.x);
+    }
+    s_total[threadIdx.x] = total;
+  }
+  const long long padded = threadIdx.x < E_local ? (static_cast<long long>(total) + align - 1) / align * align : 0;
+  int incl = static_cast<int>(padded);   // a sum of padded segments fits: checked by the host
+  if (threadIdx.x < E_GLOBAL) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += o;
+    }
+    if (lane == 31) s_scan[warp] = incl;
+  }
+  __syncthreads();
+  if (threadIdx.x < E_GLOBAL) {
+    for (int w = 0; w < warp; ++w) incl += s_scan[w];
+    s_begin[threadIdx.x + 1] = incl;
+    s_next[threadIdx.x] = incl - static_cast<int>(padded) + before;
+    if (threadIdx.x == 0) s_begin[0] = 0;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    if (threadIdx.x < E_local) counts[threadIdx.x] = s_total[threadIdx.x];
+    if (threadIdx.x <= E_local) offsets[threadIdx.x] = min(s_begin[threadIdx.x], rows);
+  }
+  // rows without a pair: the ends of the segments and what lies behind the last
+  for (int e = blockIdx.x * SORT_WARPS + warp; e < E_local; e += gridDim.x * SORT_WARPS)
+    for (int r = s_begin[e] + s_total[e] + lane; r < min(s_begin[e + 1], rows); r += 32) row_pairs[r] = -1;
+  for (long long r = s_begin[E_local] + static_cast<long long>(blockIdx.x) * SORT_THREADS + threadIdx.x; r < rows;
+       r += static_cast<long long>(gridDim.x) * SORT_THREADS)
+    row_pairs[r] = -1;
+
+  const long long first = blockIdx.x * per;
+  for (long long i = 0; i < per; i += SORT_THREADS) {
+    for (int j = threadIdx.x; j < SORT_WARPS * E_GLOBAL; j += SORT_THREADS) (&s_warp[0][0])[j] = 0;
+    __syncthreads();
+    const long long p = first + i + threadIdx.x;
+    const int e = i + threadIdx.x < per ? local_expert(topk_idx, p, n_pairs, offset, E_local) : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, e);
+    const int rank = __popc(same & ((1u << lane) - 1u));
+    if (e >= 0 && rank == 0) s_warp[warp][e] = static_cast<uint16_t>(__popc(same));
+    __syncthreads();
+    if (threadIdx.x < E_local) {
+      int run = 0;
+      for (int w = 0; w < SORT_WARPS; ++w) {
+        const int c = s_warp[w][threadIdx.x];
+        s_warp[w][threadIdx.x] = static_cast<uint16_t>(run);
+        run += c;
+      }
+      s_total[threadIdx.x] = run;   // of this round
+    }
+    __syncthreads();
+    if (p < n_pairs && i + threadIdx.x < per) {
+      int row = -1;
+      if (e >= 0) {
+        row = s_next[e] + s_warp[warp][e] + rank;
+        if (row >= rows) row = -1;
+      }
+      scatter_map[p] = row;
+      if (row >= 0) row_pairs[row] = static_cast<int>(p);
+    }
+    __syncthreads();
+    if (threadIdx.x < E_local) s_next[threadIdx.x] += s_total[threadIdx.x];
+  }
+}
+
+// The rows of token t's pairs; an entry outside 0 .. rows - 1 is none (-1), so that a map of another batch cannot lead a store
+// out of the buffer.
+__device__ __forceinline__ bool token_rows(const int* scatter_map, long long t, int K, int rows, int (&row)[TOP_K]) {
+  bool any = false;
+#pragma unroll
+  for (int k = 0; k < TOP_K; ++k) {
+    row[k] = k < K ? ld_dep(scatter_map + t * K + k) : -1;
+    if (static_cast<uint32_t>(row[k]) >= static_cast<uint32_t>(rows)) row[k] = -1;
+    any |= row[k] >= 0;
+  }
+  return any;
+}
+
+// CTA i's share of the rows is looked through for rows without a pair, which become zeros.
+__device__ __forceinline__ void zero_unused_rows(const int* row_pairs, int rows, uint8_t* out, int pieces) {
+  const int begin = static_cast<int>(static_cast<long long>(rows) * blockIdx.x / gridDim.x);
+  const int end = static_cast<int>(static_cast<long long>(rows) * (blockIdx.x + 1) / gridDim.x);
+  for (int r = begin; r < end; ++r) {
+    if (ld_dep(row_pairs + r) >= 0) continue;
+    uint4* dst = reinterpret_cast<uint4*>(out) + static_cast<long long>(r) * pieces;
+    for (int p = threadIdx.x; p < pieces; p += blockDim.x) dst[p] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// out[row(t,k)] = x[t]; one CTA per token, which also zeroes its share of the unused rows.
+__global__ void __launch_bounds__(256)
+k_token_gather(const uint8_t* x, long long x_pitch, int T, int K, int rows, int pieces, const int* row_pairs,
+               const int* scatter_map, uint8_t* out) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int t = blockIdx.x;
+  if (t < T) {
+    int row[TOP_K];
+    const bool any = token_rows(scatter_map, t, K, rows, row);
+    const uint4* src = reinterpret_cast<const uint4*>(x + t * x_pitch);
+    for (int p = threadIdx.x; any && p < pieces; p += blockDim.x) {
+      const uint4 v = ld_dep(src + p);
+#pragma unroll
+      for (int k = 0; k < TOP_K; ++k)
+        if (row[k] >= 0) reinterpret_cast<uint4*>(out)[static_cast<long long>(row[k]) * pieces + p] = v;
+    }
+  }
+  zero_unused_rows(row_pairs, rows, out, pieces);
+}
+
+// out[t] = sum_k w[t,k] * in[row(t,k)], k ascending (weights == nullptr: 1); one CTA per token.
+template <typename X>
+__global__ void __launch_bounds__(256)
+k_token_combine(const uint8_t* in, long long in_pitch, const float* weights, int K, int rows, int pieces,
+                const int* scatter_map, uint8_t* out) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int N = PIECE_ELEMS<X>;
+  const int t = blockIdx.x;
+  int row[TOP_K];
+  float w[TOP_K];
+  token_rows(scatter_map, t, K, rows, row);
+#pragma unroll
+  for (int k = 0; k < TOP_K; ++k) w[k] = k < K && weights ? ld_dep(weights + static_cast<long long>(t) * K + k) : 1.f;
+  for (int p = threadIdx.x; p < pieces; p += blockDim.x) {
+    uint4 raw[TOP_K];
+#pragma unroll
+    for (int k = 0; k < TOP_K; ++k)
+      if (row[k] >= 0) raw[k] = ld_dep(reinterpret_cast<const uint4*>(in + row[k] * in_pitch) + p);
+    float acc[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) acc[j] = 0.f;
+#pragma unroll
+    for (int k = 0; k < TOP_K; ++k) {
+      if (row[k] < 0) continue;
+      float f[N];
+      unpack_piece<X>(raw[k], f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[j] = fmaf(w[k], f[j], acc[j]);
+    }
+    reinterpret_cast<uint4*>(out)[static_cast<long long>(t) * pieces + p] = pack_piece<X>(acc);
+  }
+}
+
+// grad_in[row(t,k)] = w[t,k] * grad[t] and grad_w[t,k] = <grad[t], in[row(t,k)]> in one pass; either output may be absent.
+template <typename X>
+__global__ void __launch_bounds__(256)
+k_token_combine_backward(const uint8_t* grad, long long grad_pitch, const uint8_t* in, long long in_pitch,
+                         const float* weights, int T, int K, int rows, int pieces, const int* row_pairs,
+                         const int* scatter_map, uint8_t* grad_in, float* grad_w) {
+  __shared__ float s_dot[TOP_K][8];
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int N = PIECE_ELEMS<X>;
+  const int t = blockIdx.x;
+  if (t < T) {
+    int row[TOP_K];
+    float w[TOP_K], dot[TOP_K];
+    token_rows(scatter_map, t, K, rows, row);
+#pragma unroll
+    for (int k = 0; k < TOP_K; ++k) {
+      w[k] = k < K ? ld_dep(weights + static_cast<long long>(t) * K + k) : 0.f;
+      dot[k] = 0.f;
+    }
+    for (int p = threadIdx.x; p < pieces; p += blockDim.x) {
+      const uint4 raw_g = ld_dep(reinterpret_cast<const uint4*>(grad + t * grad_pitch) + p);
+      uint4 raw[TOP_K];
+#pragma unroll
+      for (int k = 0; k < TOP_K; ++k)
+        if (grad_w && row[k] >= 0) raw[k] = ld_dep(reinterpret_cast<const uint4*>(in + row[k] * in_pitch) + p);
+      float g[N];
+      unpack_piece<X>(raw_g, g);
+#pragma unroll
+      for (int k = 0; k < TOP_K; ++k) {
+        if (row[k] < 0) continue;
+        if (grad_w) {
+          float f[N];
+          unpack_piece<X>(raw[k], f);
+#pragma unroll
+          for (int j = 0; j < N; ++j) dot[k] = fmaf(g[j], f[j], dot[k]);
+        }
+        if (grad_in) {
+          float d[N];
+#pragma unroll
+          for (int j = 0; j < N; ++j) d[j] = w[k] * g[j];
+          reinterpret_cast<uint4*>(grad_in)[static_cast<long long>(row[k]) * pieces + p] = pack_piece<X>(d);
+        }
+      }
+    }
+    if (grad_w) {
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1)
+#pragma unroll
+        for (int k = 0; k < TOP_K; ++k) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], d);
+      if ((threadIdx.x & 31) == 0)
+#pragma unroll
+        for (int k = 0; k < TOP_K; ++k) s_dot[k][threadIdx.x >> 5] = dot[k];
+      __syncthreads();
+      if (threadIdx.x < K) {
+        float sum = 0.f;
+        for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) sum += s_dot[threadIdx.x][i];
+        grad_w[static_cast<long long>(t) * K + threadIdx.x] = sum;
+      }
+    }
+  }
+  if (grad_in) zero_unused_rows(row_pairs, rows, grad_in, pieces);
+}
+
+// w[t,k] = scale * s_k / (sum_j s_j + 1e-20) over the token's K selected experts, s = sigmoid(logit): the operations, and their
+// order, of route_token, so that the weights of a selection made by b200moe_route_topk are its bits.  Eight lanes per token.
+// An id outside 0 .. 255 has weight 0 and takes no part; a NaN logit makes its token's weights NaN (the sigmoid's clamp would
+// take it for a large one, as the routing kernels do).
+__device__ __forceinline__ float selected_sigmoid(const float* logits, long long t, int id, float sign) {
+  if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(E_GLOBAL)) return 0.f;
+  const float x = sign * ld_dep(logits + t * E_GLOBAL + id);
+  return isnan(x) ? x : sigmoid_exact_ops(x);
+}
+__global__ void __launch_bounds__(256)
+k_route_weights(const float* logits, const int* topk_idx, int T, int K, float scale, float* weights) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long t = static_cast<long long>(blockIdx.x) * (blockDim.x / TOP_K) + threadIdx.x / TOP_K;
+  const int k = threadIdx.x % TOP_K;
+  const bool live = t < T && k < K;
+  const int id = live ? ld_dep(topk_idx + t * K + k) : -1;
+  const float s = live ? selected_sigmoid(logits, t, id, 1.f) : 0.f;
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < TOP_K; ++j) sum = __fadd_rn(sum, __shfl_sync(0xffffffffu, s, j, TOP_K));
+  if (live) weights[t * K + k] = __fmul_rn(__fdiv_rn(s, __fadd_rn(sum, 1e-20f)), scale);
+}
+
+// With S = sum_j s_j + 1e-20 and g = the weights' gradient:
+//   grad_logit_k = s_k * (1 - s_k) * scale / S * (g_k - sum_j g_j s_j / S),  every other column 0.
+// 1 - sigmoid(x) is taken as sigmoid(-x), which loses nothing where s is near 1.  A warp per token; an expert named twice gets
+// both terms, in the order of k.
+__global__ void __launch_bounds__(256)
+k_route_weights_backward(const float* logits, const int* topk_idx, const float* grad, int T, int K, float scale,
+                         float* grad_logits) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const long long t = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (t >= T) return;
+  const int id = lane < K ? ld_dep(topk_idx + t * K + lane) : -1;
+  const float g = lane < K ? ld_dep(grad + t * K + lane) : 0.f;
+  const float s = selected_sigmoid(logits, t, id, 1.f), c = selected_sigmoid(logits, t, id, -1.f);
+  float total = s, mix = static_cast<uint32_t>(id) < static_cast<uint32_t>(E_GLOBAL) ? g * s : 0.f;
+#pragma unroll
+  for (int d = 4; d > 0; d >>= 1) {   // lanes 0..7
+    total += __shfl_xor_sync(0xffffffffu, total, d);
+    mix += __shfl_xor_sync(0xffffffffu, mix, d);
+  }
+  total += 1e-20f;
+  const float grad_k = s * c * (scale / total) * (g - mix / total);
+  float out[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) out[j] = 0.f;
+#pragma unroll
+  for (int k = 0; k < TOP_K; ++k) {
+    const int e = __shfl_sync(0xffffffffu, id, k);
+    const float d = __shfl_sync(0xffffffffu, grad_k, k);
+    if (static_cast<uint32_t>(e) >= static_cast<uint32_t>(E_GLOBAL)) continue;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)   // column 4 * lane + 128 * (j / 4) + j % 4
+      if (e == 4 * lane + 128 * (j >> 2) + (j & 3)) out[j] += d;
+  }
+  float4* dst = reinterpret_cast<float4*>(grad_logits + t * E_GLOBAL);
+  dst[lane] = make_float4(out[0], out[1], out[2], out[3]);
+  dst[32 + lane] = make_float4(out[4], out[5], out[6], out[7]);
+}
+
+// Pairs per CTA and CTAs of the sort: whole rounds of SORT_THREADS pairs, at most SORT_MAX_CTAS CTAs.
+static long long sort_pairs_per_cta(long long n_pairs) {
+  const long long rounds = (n_pairs + SORT_THREADS - 1) / SORT_THREADS;
+  const long long per = (rounds + SORT_MAX_CTAS - 1) / SORT_MAX_CTAS;
+  return (per < 1 ? 1 : per) * SORT_THREADS;
+}
+
+size_t token_sort_scratch_bytes(int T, int K, int E_local) {
+  const long long n_pairs = static_cast<long long>(T) * K;
+  const long long per = sort_pairs_per_cta(n_pairs);
+  return static_cast<size_t>(n_pairs == 0 ? 1 : (n_pairs + per - 1) / per) * E_local * sizeof(int);
+}
+
+int launch_token_sort(const int* topk_idx, int T, int K, int E_local, int offset, int align, int rows, int* hist,
+                      int* counts, int* offsets, int* row_pairs, int* scatter_map, cudaStream_t st) {
+  const long long n_pairs = static_cast<long long>(T) * K;
+  const long long per = sort_pairs_per_cta(n_pairs);
+  const unsigned ctas = n_pairs == 0 ? 1u : static_cast<unsigned>((n_pairs + per - 1) / per);
+  B200MOE_CUDA_TRY(launch_pdl(k_token_count, dim3(ctas), dim3(SORT_THREADS), 0, st, topk_idx, n_pairs, per, offset, E_local,
+                              hist));
+  B200MOE_CUDA_TRY(launch_pdl(k_token_place, dim3(ctas), dim3(SORT_THREADS), 0, st, topk_idx, n_pairs, per, offset, E_local,
+                              align, rows, static_cast<const int*>(hist), counts, offsets, row_pairs, scatter_map));
+  return B200MOE_OK;
+}
+
+// One CTA per token, more where the capacity has many rows per token.
+static unsigned token_ctas(int T, int rows) {
+  const int by_rows = (rows + TOP_K - 1) / TOP_K;
+  return static_cast<unsigned>(T > by_rows ? T : by_rows);
+}
+static unsigned token_threads(int pieces) {
+  const int threads = (pieces + 31) / 32 * 32;
+  return static_cast<unsigned>(threads < 256 ? threads : 256);
+}
+
+int launch_token_gather(const void* x, long long x_pitch, int T, int K, int rows, int pieces, const int* row_pairs,
+                        const int* scatter_map, void* out, cudaStream_t st) {
+  B200MOE_CUDA_TRY(launch_pdl(k_token_gather, dim3(token_ctas(T, rows)), dim3(token_threads(pieces)), 0, st,
+                              static_cast<const uint8_t*>(x), x_pitch, T, K, rows, pieces, row_pairs, scatter_map,
+                              static_cast<uint8_t*>(out)));
+  return B200MOE_OK;
+}
+
+template <typename F>
+static int with_row_type(int type, F&& f) {
+  if (type == B200MOE_DTYPE_F32) return f(float());
+  if (type == B200MOE_DTYPE_F16) return f(__half());
+  return f(__nv_bfloat16());
+}
+
+int launch_token_combine(const void* in, long long in_pitch, int type, const float* weights, int T, int K, int rows,
+                         int pieces, const int* scatter_map, void* out, cudaStream_t st) {
+  return with_row_type(type, [&](auto xt) -> int {
+    B200MOE_CUDA_TRY(launch_pdl(k_token_combine<decltype(xt)>, dim3(T), dim3(token_threads(pieces)), 0, st,
+                                static_cast<const uint8_t*>(in), in_pitch, weights, K, rows, pieces, scatter_map,
+                                static_cast<uint8_t*>(out)));
+    return B200MOE_OK;
+  });
+}
+
+int launch_token_combine_backward(const void* grad, long long grad_pitch, const void* in, long long in_pitch, int type,
+                                  const float* weights, int T, int K, int rows, int pieces, const int* row_pairs,
+                                  const int* scatter_map, void* grad_in, float* grad_w, cudaStream_t st) {
+  return with_row_type(type, [&](auto xt) -> int {
+    B200MOE_CUDA_TRY(launch_pdl(k_token_combine_backward<decltype(xt)>, dim3(grad_in ? token_ctas(T, rows) : T),
+                                dim3(token_threads(pieces)), 0, st, static_cast<const uint8_t*>(grad), grad_pitch,
+                                static_cast<const uint8_t*>(in), in_pitch, weights, T, K, rows, pieces, row_pairs,
+                                scatter_map, static_cast<uint8_t*>(grad_in), grad_w));
+    return B200MOE_OK;
+  });
+}
+
+int launch_route_weights(const float* logits, const int* topk_idx, int T, int K, float scale, float* weights,
+                         cudaStream_t st) {
+  B200MOE_CUDA_TRY(launch_pdl(k_route_weights, dim3((T + 31) / 32), dim3(256), 0, st, logits, topk_idx, T, K, scale,
+                              weights));
+  return B200MOE_OK;
+}
+
+int launch_route_weights_backward(const float* logits, const int* topk_idx, const float* grad, int T, int K, float scale,
+                                  float* grad_logits, cudaStream_t st) {
+  B200MOE_CUDA_TRY(launch_pdl(k_route_weights_backward, dim3((T + 7) / 8), dim3(256), 0, st, logits, topk_idx, grad, T, K,
+                              scale, grad_logits));
+  return B200MOE_OK;
+}
+
+}  // namespace b200moe

@@ -1,0 +1,82 @@
+"""What the operators around the layer (``norm``, ``tokens``) share: checks of row tensors, their way to the C ABI, and the rule
+on stream capture."""
+from __future__ import annotations
+
+import contextlib
+from typing import Tuple
+
+import torch
+
+from . import _lib
+from .kernel import _require_cuda
+
+DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
+MAX_TOKENS = 1 << 24
+
+
+def check_rows(t, name: str) -> Tuple[int, int]:
+    """(rows, columns) of a 2-d tensor of bf16, f16 or f32."""
+    if not torch.is_tensor(t):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype not in DTYPES:
+        raise TypeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
+    if t.dim() != 2:
+        raise ValueError(f"{name} must have two dimensions, got {tuple(t.shape)}")
+    return int(t.shape[0]), int(t.shape[1])
+
+
+def check_tensor(t, name: str, dtype: torch.dtype, shape: Tuple[int, ...]) -> None:
+    if not torch.is_tensor(t):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+
+
+def check_device(first: torch.Tensor, **tensors) -> None:
+    """All on the CUDA device of ``first``."""
+    device = first.device
+    if device.type != "cuda" or any(t is not None and t.device != device for t in tensors.values()):
+        _require_cuda(input=first, **tensors)
+        raise RuntimeError("all tensors must live on one device: " + ", ".join(
+            f"{n} is on {t.device}" for n, t in tensors.items() if t is not None) + f", the input on {device}")
+
+
+def row_pointer(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """A tensor whose rows the library can read in place and their distance in bytes (0 = dense): ``t`` itself where its rows are
+    dense, 16-byte aligned and apart, else a copy.  The caller keeps the tensor until the launch."""
+    size = t.element_size()
+    if t.is_contiguous():
+        return (t if t.data_ptr() % 16 == 0 else t.clone()), 0
+    pitch = t.stride(0) * size
+    if t.stride(1) == 1 and t.stride(0) >= t.shape[1] and pitch % 16 == 0 and t.data_ptr() % 16 == 0:
+        return t, pitch
+    return t.contiguous(), 0
+
+
+def dense(t: torch.Tensor, align: int = 4) -> torch.Tensor:
+    """``t`` if it is contiguous and its address a multiple of ``align``, else a copy."""
+    t = t.contiguous()
+    return t if t.data_ptr() % align == 0 else t.clone()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def records_graph(instead: str, *tensors) -> bool:
+    """Whether a call on these tensors has to record an autograd node.  During stream capture that is refused: where an eager
+    graph over the same leaves is alive, their accumulation nodes belong to another stream than the captured one, and running
+    them under capture ends the process.  ``instead`` names the function that computes the gradient explicitly."""
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+        return False
+    refuse_capture(instead)
+    return True
+
+
+def refuse_capture(instead: str) -> None:
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("autograd is not available during stream capture: capture the call under torch.no_grad() and "
+                           f"its gradient as {instead}(...)")

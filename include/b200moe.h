@@ -199,6 +199,76 @@ int b200moe_forward(const b200moe_problem* p /* host */, const b200moe_workspace
  * with 448 / amax, scripts/yjl_ncu.py:413-416).  x_bf16 16-byte aligned, q_out 8-byte aligned; needs no workspace. */
 int b200moe_quantize_act(const void* x_bf16, int32_t T, void* q_out, float* scale_out, void* stream);
 
+/* ---- Around the layer (no reference counterpart: the reference takes quantised activations and returns rows) ----------
+ * Element types of rows.  Rows are `columns` elements; a *_pitch is the distance between two rows in bytes (a multiple of 16;
+ * 0 = dense), rows without one are dense.  Row pointers are 16-byte aligned. */
+#define B200MOE_DTYPE_BF16 0
+#define B200MOE_DTYPE_F16 1
+#define B200MOE_DTYPE_F32 2
+#define B200MOE_NORM_MAX_COLUMNS 16384
+
+/* Residual addition and RMS norm, with the layer's quantisation on the way out:
+ *   r = x + residual, rounded to residual_type          (residual NULL: r = x, stream_out is not written)
+ *   y = r * weight / sqrt(mean(r^2) + eps)              float32 arithmetic on the rounded r
+ * stream_out [T, columns] of residual_type receives r (it may be `residual` itself); y_out (optional) y in x_type; q_out and
+ * scale_out (optional, together) e4m3 rows and their float32 scales [columns / 128, T] by the rule of b200moe_quantize_act,
+ * applied to the float32 y; a NaN in a block makes its scale NaN.
+ * columns: a multiple of 8 (of 128 with q_out), at most B200MOE_NORM_MAX_COLUMNS; residual_type: x_type or float32;
+ * weight [columns] of any type. */
+int b200moe_add_rms_norm(const void* x, int64_t x_pitch, int32_t x_type, const void* residual, int64_t residual_pitch,
+                         int32_t residual_type, const void* weight, int32_t weight_type, int32_t T, int32_t columns,
+                         float eps, void* stream_out, void* y_out, void* q_out, float* scale_out, void* stream);
+/* Its gradient.  grad_y [T, columns] of `type`, grad_stream (optional) and stream_rows = the r of the forward call of stream_type:
+ *   dr = (g - r * mean(g * r) / v) / sqrt(v) + grad_stream,   g = grad_y * weight,  v = mean(r^2) + eps
+ * grad_x (optional) receives dr in `type`, grad_residual (optional) in stream_type, grad_weight (optional) the sum over tokens of
+ * grad_y * r / sqrt(v) in weight_type.  With grad_weight, `partial` is scratch of min(T, B200MOE_NORM_PARTIAL_ROWS) rows
+ * of `columns` floats.  Every sum has a fixed order: the same call gives the same bits. */
+#define B200MOE_NORM_PARTIAL_ROWS 512
+int b200moe_add_rms_norm_backward(const void* grad_y, int64_t grad_y_pitch, int32_t type, const void* grad_stream,
+                                  int64_t grad_stream_pitch, const void* stream_rows, int64_t stream_pitch,
+                                  int32_t stream_type, const void* weight, int32_t weight_type, int32_t T, int32_t columns,
+                                  float eps, void* grad_x, void* grad_residual, void* grad_weight, float* partial,
+                                  void* stream);
+
+/* Tokens sorted by expert, for experts that are the caller's own products (training, other weights than the layer's).
+ * topk_idx [T, K], K <= 8: ids outside [offset, offset + E_local) take no part (-1 for the padding of a batch), and a token may
+ * name an expert twice.  Pair p = t * K + k gets row offsets[e] + (pairs of expert e before p); every segment starts at a multiple
+ * of `align`; a pair whose row would be `rows` (the capacity) or more gets none.  T * K + E_local * (align - 1) and `rows` are at most B200MOE_TOKEN_MAX_ROWS.
+ *   counts [E_local]       pairs of each local expert, those without a row among them
+ *   offsets [E_local + 1]  first row of each segment and the end of the last, at most `rows`
+ *   row_pairs [rows]       pair of each row, -1 for a row without one
+ *   scatter_map [T, K]     row of each pair, -1 for a pair without one
+ * scratch: b200moe_token_sort_scratch_bytes(T, K, E_local) bytes, 4-byte aligned, not shared with a call in flight. */
+#define B200MOE_TOKEN_SORT_MAX_CTAS 256
+#define B200MOE_TOKEN_MAX_ROWS (1 << 30)
+int b200moe_token_sort_scratch_bytes(int32_t T, int32_t K, int32_t E_local, size_t* bytes /* host */);
+int b200moe_token_sort(const int32_t* topk_idx, int32_t T, int32_t K, int32_t E_local, int32_t offset, int32_t align,
+                       int32_t rows, void* scratch, size_t scratch_bytes, int32_t* counts, int32_t* offsets,
+                       int32_t* row_pairs, int32_t* scatter_map, void* stream);
+/* out[row(t,k)] = x[t] for every pair with a row; the other rows become zeros.  columns * element size: a multiple of 16. */
+int b200moe_token_gather(const void* x, int64_t x_pitch, int32_t type, int32_t T, int32_t K, int32_t columns, int32_t rows,
+                         const int32_t* row_pairs, const int32_t* scatter_map, void* out, void* stream);
+/* out[t] = sum over k of weights[t,k] * rows_in[row(t,k)], k ascending, float32 sums, rounded once; zeros for a token without a row.
+ * weights NULL: 1, which is the gradient of b200moe_token_gather.  An entry of a map outside 0 .. rows - 1 counts as -1 in all of
+ * these calls. */
+int b200moe_token_combine(const void* rows_in, int64_t rows_pitch, int32_t type, const float* weights, int32_t T, int32_t K,
+                          int32_t columns, int32_t rows, const int32_t* scatter_map, void* out, void* stream);
+/* Gradient of b200moe_token_combine: grad_rows[row(t,k)] = weights[t,k] * grad[t], zeros in the other rows (optional);
+ * grad_weights[t,k] = sum over columns of grad[t] * rows_in[row(t,k)], 0 for a pair without a row (optional; rows_in may be NULL
+ * without it). */
+int b200moe_token_combine_backward(const void* grad, int64_t grad_pitch, const void* rows_in, int64_t rows_pitch,
+                                   int32_t type, const float* weights, int32_t T, int32_t K, int32_t columns, int32_t rows,
+                                   const int32_t* row_pairs, const int32_t* scatter_map, void* grad_rows,
+                                   float* grad_weights, void* stream);
+/* Weights of selected experts: weights[t,k] = scale * s_k / (sum_j s_j + 1e-20), s = sigmoid(logits[t, topk_idx[t,k]]), the bits that
+ * b200moe_route_topk gives for its own selection; ids outside 0..255 have weight 0 and take no part;
+ * a NaN logit makes its token's weights NaN.  And the gradient with respect to the logits [T, 256], every element of which
+ * is written. */
+int b200moe_route_weights(const float* logits, const int32_t* topk_idx, int32_t T, int32_t K, float scale, float* weights,
+                          void* stream);
+int b200moe_route_weights_backward(const float* logits, const int32_t* topk_idx, const float* grad_weights, int32_t T,
+                                   int32_t K, float scale, float* grad_logits, void* stream);
+
 /* Stage entry points (unit tests, profiling).  Each runs one stage of b200moe_forward on the same buffers. */
 
 /* No-aux routing: sigmoid, +bias, group score = two largest of each 32-expert group, top-4 groups, top-8 experts,

@@ -17,6 +17,10 @@ namespace b200moe {
 constexpr int SORT_THREADS = 1024;   // pairs ranked at once by a CTA
 constexpr int SORT_WARPS = SORT_THREADS / 32;
 constexpr int SORT_MAX_CTAS = B200MOE_TOKEN_SORT_MAX_CTAS;
+#ifndef B200MOE_SORT_ONE_LAUNCH_CTAS
+#define B200MOE_SORT_ONE_LAUNCH_CTAS 16
+#endif
+constexpr unsigned SORT_ONE_LAUNCH_CTAS = B200MOE_SORT_ONE_LAUNCH_CTAS;
 
 // Index of the pair's local expert, or -1.  Unsigned: a negative id is a large one.
 __device__ __forceinline__ int local_expert(const int* topk_idx, long long p, long long n_pairs, int offset, int E_local) {
@@ -42,7 +46,8 @@ k_token_count(const int* topk_idx, long long n_pairs, long long per, int offset,
   if (threadIdx.x < E_local) hist[blockIdx.x * E_local + threadIdx.x] = s_count[threadIdx.x];
 }
 
-// The rows: every CTA derives the layout from the counts of all CTAs, then ranks its pairs SORT_THREADS at a time.  Inside a
+// The rows: every CTA derives the layout from the counts of all CTAs (`hist`, or for a small batch, hist == nullptr, by counting
+// the whole batch itself, which saves the launch of k_token_count), then ranks its pairs SORT_THREADS at a time.  Inside a
 // warp the rank is the number of lower lanes with the same expert, and the warps' counts are prefixed per expert.
 __global__ void __launch_bounds__(SORT_THREADS)
 k_token_place(const int* topk_idx, long long n_pairs, long long per, int offset, int E_local, int align, int rows,
@@ -56,7 +61,23 @@ k_token_place(const int* topk_idx, long long n_pairs, long long per, int offset,
   pdl_launch_dependents();
   pdl_wait();
   int total = 0, before = 0;
-  if (threadIdx.x < E_local) {
+  if (!hist) {
+    int* s_before = &s_next[0];
+    if (threadIdx.x < E_GLOBAL) s_total[threadIdx.x] = s_before[threadIdx.x] = 0;
+    __syncthreads();
+    const long long mine = blockIdx.x * per;
+    for (long long p = threadIdx.x; p < n_pairs; p += SORT_THREADS) {
+      const int e = local_expert(topk_idx, p, n_pairs, offset, E_local);
+      if (e < 0) continue;
+      atomicAdd(&s_total[e], 1);
+      if (p < mine) atomicAdd(&s_before[e], 1);
+    }
+    __syncthreads();
+    if (threadIdx.x < E_local) {
+      total = s_total[threadIdx.x];
+      before = s_before[threadIdx.x];
+    }
+  } else if (threadIdx.x < E_local) {
     for (int b = 0; b < static_cast<int>(gridDim.x); ++b) {
       if (b == static_cast<int>(blockIdx.x)) before = total;
       total += ld_dep(hist + b * E_local + threadIdx.x);
@@ -351,8 +372,12 @@ int launch_token_sort(const int* topk_idx, int T, int K, int E_local, int offset
   const long long n_pairs = static_cast<long long>(T) * K;
   const long long per = sort_pairs_per_cta(n_pairs);
   const unsigned ctas = n_pairs == 0 ? 1u : static_cast<unsigned>((n_pairs + per - 1) / per);
-  B200MOE_CUDA_TRY(launch_pdl(k_token_count, dim3(ctas), dim3(SORT_THREADS), 0, st, topk_idx, n_pairs, per, offset, E_local,
-                              hist));
+  if (ctas <= SORT_ONE_LAUNCH_CTAS) {
+    hist = nullptr;
+  } else {
+    B200MOE_CUDA_TRY(launch_pdl(k_token_count, dim3(ctas), dim3(SORT_THREADS), 0, st, topk_idx, n_pairs, per, offset,
+                                E_local, hist));
+  }
   B200MOE_CUDA_TRY(launch_pdl(k_token_place, dim3(ctas), dim3(SORT_THREADS), 0, st, topk_idx, n_pairs, per, offset, E_local,
                               align, rows, static_cast<const int*>(hist), counts, offsets, row_pairs, scatter_map));
   return B200MOE_OK;

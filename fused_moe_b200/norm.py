@@ -10,11 +10,10 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .rows import DTYPES, MAX_TOKENS, check_device, check_rows, check_tensor, dense, on_device, records_graph, \
-    refuse_capture, row_pointer
+from .rows import DTYPES, MAX_TOKENS, check_device, check_rows, check_tensor, dense, differentiable_once, on_device, \
+    records_graph, refuse_capture, row_pointer, stream_of
 
 QBLOCK = 128
 _FP8 = torch.float8_e4m3fn
@@ -53,7 +52,7 @@ def _forward(x, residual, weight, eps, stream, y, q, scale) -> None:
             DTYPES[x.dtype if rr is None else rr.dtype], w.data_ptr(), DTYPES[w.dtype], T, columns, eps,
             None if rr is None else stream.data_ptr(), None if y is None else y.data_ptr(),
             None if q is None else q.data_ptr(), None if scale is None else scale.data_ptr(),
-            torch.cuda.current_stream(device).cuda_stream), "b200moe_add_rms_norm")
+            stream_of(device)), "b200moe_add_rms_norm")
 
 
 def _backward(grad_y, grad_stream, stream, weight, eps, need_x: bool, need_residual: bool, need_weight: bool):
@@ -62,17 +61,16 @@ def _backward(grad_y, grad_stream, stream, weight, eps, need_x: bool, need_resid
     T, columns = stream.shape
     device = stream.device
     one = grad_y.dtype is stream.dtype
-    empty = lambda dtype: torch.empty((T, columns), dtype=dtype, device=device)  # noqa: E731
-    grad_x = empty(grad_y.dtype) if need_x or (one and need_residual) else None
-    grad_residual = grad_x if one else empty(stream.dtype) if need_residual else None
+    grad_x = grad_y.new_empty((T, columns)) if need_x or (one and need_residual) else None
+    grad_residual = grad_x if one else stream.new_empty((T, columns)) if need_residual else None
     grad_weight = None
     if T == 0:
         grad_weight = torch.zeros(columns, dtype=weight.dtype, device=device) if need_weight else None
     else:
         partial = None
         if need_weight:
-            grad_weight = torch.empty(columns, dtype=weight.dtype, device=device)
-            partial = torch.empty((min(T, _lib.NORM_PARTIAL_ROWS), columns), dtype=torch.float32, device=device)
+            grad_weight = weight.new_empty(columns)
+            partial = weight.new_empty((min(T, _lib.NORM_PARTIAL_ROWS), columns), dtype=torch.float32)
         gy, gy_pitch = row_pointer(grad_y)
         gs, gs_pitch = (None, 0) if grad_stream is None else row_pointer(grad_stream)
         rr, r_pitch = row_pointer(stream)
@@ -84,15 +82,15 @@ def _backward(grad_y, grad_stream, stream, weight, eps, need_x: bool, need_resid
                 None if grad_x is None else grad_x.data_ptr(),
                 None if one or grad_residual is None else grad_residual.data_ptr(),
                 None if grad_weight is None else grad_weight.data_ptr(), None if partial is None else partial.data_ptr(),
-                torch.cuda.current_stream(device).cuda_stream), "b200moe_add_rms_norm_backward")
+                stream_of(device)), "b200moe_add_rms_norm_backward")
     return grad_x if need_x else None, grad_residual if need_residual else None, grad_weight
 
 
 class _AddRmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        stream = None if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+        y = x.new_empty(x.shape)
+        stream = None if residual is None else residual.new_empty(x.shape)
         _forward(x, residual, weight, eps, stream, y, None, None)
         ctx.save_for_backward(x if residual is None else stream, weight)
         ctx.eps, ctx.x_dtype = eps, x.dtype
@@ -100,7 +98,7 @@ class _AddRmsNorm(torch.autograd.Function):
         return y if residual is None else (y, stream)
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, grad_y, grad_stream=None):
         refuse_capture("add_rms_norm_backward")
         stream, weight = ctx.saved_tensors
@@ -123,18 +121,17 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
     the weight only, and its sums have a fixed order.  During stream capture a call that would record a gradient is
     refused (``add_rms_norm_backward`` is the explicit form)."""
     T, columns = _check(x, residual, weight, eps, 8)
-    check_device(x, residual=residual, weight=weight)
+    check_device(x, residual, weight)
     if records_graph("add_rms_norm_backward", x, residual, weight):
         if residual is None:
             return _AddRmsNorm.apply(x, None, weight, eps), x
         return _AddRmsNorm.apply(x, residual, weight, eps)
-    y = torch.empty((T, columns), dtype=x.dtype, device=x.device)
-    stream = x if residual is None else torch.empty((T, columns), dtype=residual.dtype, device=x.device)
+    y = x.new_empty((T, columns))
+    stream = x if residual is None else residual.new_empty((T, columns))
     _forward(x, residual, weight, eps, stream, y, None, None)
     return y, stream
 
 
-@torch.no_grad()
 def add_rms_norm_backward(grad_y: torch.Tensor, grad_stream: Optional[torch.Tensor], stream: torch.Tensor,
                           weight: torch.Tensor, eps: float = 1e-6):
     """Gradients (grad_x, grad_residual, grad_weight) of ``add_rms_norm`` from those of its results: ``grad_y`` and, unless
@@ -146,11 +143,10 @@ def add_rms_norm_backward(grad_y: torch.Tensor, grad_stream: Optional[torch.Tens
     shape = _check(grad_y, stream, weight, eps, 8, ("grad_y", "stream"))
     if grad_stream is not None:
         check_tensor(grad_stream, "grad_stream", stream.dtype, shape)
-    check_device(grad_y, stream=stream, weight=weight, grad_stream=grad_stream)
+    check_device(grad_y, stream, weight, grad_stream)
     return _backward(grad_y, grad_stream, stream, weight, eps, True, True, True)
 
 
-@torch.no_grad()
 def add_rms_norm_quantize(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-6, *,
                           residual_out: Optional[torch.Tensor] = None, with_normed: bool = False):
     """(q, scales, r) or, ``with_normed``, (q, scales, r, y): residual addition, RMS norm and the layer's quantisation in one launch.
@@ -160,26 +156,26 @@ def add_rms_norm_quantize(x: torch.Tensor, residual: Optional[torch.Tensor], wei
     the type of ``x``, which the router's product reads.  Arguments as for ``add_rms_norm`` with n a multiple of 128.
     ``residual_out`` [T, n] of the residual's type receives r and may be ``residual`` itself."""
     T, columns = _check(x, residual, weight, eps, QBLOCK)
-    check_device(x, residual=residual, weight=weight)
+    check_device(x, residual, weight)
     if residual is None:
         if residual_out is not None:
             raise ValueError("residual_out needs a residual")
         stream = x
     elif residual_out is None:
-        stream = torch.empty((T, columns), dtype=residual.dtype, device=x.device)
+        stream = residual.new_empty((T, columns))
     else:
         stream = residual_out
         check_tensor(stream, "residual_out", residual.dtype, (T, columns))
-        check_device(x, residual_out=stream)
+        check_device(x, stream)
         if not stream.is_contiguous() or stream.data_ptr() % 16:
             raise ValueError("residual_out must be contiguous and 16-byte aligned")
         for name, t in (("x", x), ("residual", residual), ("weight", weight)):
             same = t.data_ptr() == stream.data_ptr() and t.dtype is stream.dtype and t.is_contiguous() and t is not weight
             if not same and _overlap(t, stream):
                 raise ValueError(f"residual_out overlaps {name} without being it")
-    q = torch.empty((T, columns), dtype=_FP8, device=x.device)
-    scale = torch.empty((columns // QBLOCK, T), dtype=torch.float32, device=x.device)
-    y = torch.empty((T, columns), dtype=x.dtype, device=x.device) if with_normed else None
+    q = x.new_empty((T, columns), dtype=_FP8)
+    scale = x.new_empty((columns // QBLOCK, T), dtype=torch.float32)
+    y = x.new_empty((T, columns)) if with_normed else None
     _forward(x, residual, weight, eps, stream, y, q, scale)
     return (q, scale, stream, y) if with_normed else (q, scale, stream)
 

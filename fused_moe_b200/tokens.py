@@ -17,12 +17,11 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .kernel import E_GLOBAL, TOP_K, _host_scalar
-from .rows import DTYPES, MAX_TOKENS, check_device, check_rows, check_tensor, dense, on_device, records_graph, \
-    refuse_capture, row_pointer
+from .rows import DTYPES, MAX_TOKENS, check_device, check_rows, check_tensor, dense, differentiable_once, on_device, \
+    records_graph, refuse_capture, row_pointer, stream_of
 
 
 @dataclass(frozen=True)
@@ -54,7 +53,6 @@ def _selection(topk_idx) -> tuple:
     return int(topk_idx.shape[0]), int(topk_idx.shape[1])
 
 
-@torch.no_grad()
 def sort_tokens(topk_idx: torch.Tensor, E_local: int, local_expert_offset=0, align: int = 1,
                 rows: Optional[int] = None) -> TokenSort:
     """Sorts the pairs of ``topk_idx`` [T, K] int32 (K <= 8, global expert ids) stably by local expert: row of a pair = start of
@@ -78,19 +76,18 @@ def sort_tokens(topk_idx: torch.Tensor, E_local: int, local_expert_offset=0, ali
         rows = T * K if align == 1 else (T * K // align + min(E_local, T * K)) * align
     if not 0 <= rows <= _lib.TOKEN_MAX_ROWS:
         raise ValueError(f"rows must be in 0..{_lib.TOKEN_MAX_ROWS}")
-    check_device(topk_idx)
-    device = topk_idx.device
+    device = check_device(topk_idx)
     idx = dense(topk_idx)
     lib = _lib.load()
     need = C.c_size_t(0)
     _lib.check(lib.b200moe_token_sort_scratch_bytes(T, K, E_local, C.byref(need)), "b200moe_token_sort_scratch_bytes")
-    ints = lambda *shape: torch.empty(shape, dtype=torch.int32, device=device)  # noqa: E731
-    plan = TokenSort(ints(E_local), ints(E_local + 1), ints(rows), ints(T, K), rows, align)
+    ints = topk_idx.new_empty
+    plan = TokenSort(ints(E_local), ints(E_local + 1), ints(rows), ints((T, K)), rows, align)
     scratch = ints(need.value // 4)
     with on_device(device):
         _lib.check(lib.b200moe_token_sort(idx.data_ptr(), T, K, E_local, offset, align, rows, scratch.data_ptr(), need.value,
                                           plan.counts.data_ptr(), plan.offsets.data_ptr(), plan.row_pairs.data_ptr(),
-                                          plan.scatter_map.data_ptr(), torch.cuda.current_stream(device).cuda_stream),
+                                          plan.scatter_map.data_ptr(), stream_of(device)),
                    "b200moe_token_sort")
     return plan
 
@@ -103,31 +100,31 @@ def _check_batch(t, name: str, plan: TokenSort, rows: int) -> int:
         raise ValueError(f"{name} must have {rows} rows, got {n}")
     if columns == 0 or columns * t.element_size() % 16 or columns > 1 << 24:
         raise ValueError(f"a row of {name} must be a multiple of 16 bytes, got {columns} columns of {t.dtype}")
-    check_device(t, plan=plan.scatter_map)
+    check_device(t, plan.scatter_map)
     return columns
 
 
 def _gather(x: torch.Tensor, plan_rows: int, row_pairs: torch.Tensor, scatter_map: torch.Tensor) -> torch.Tensor:
     (T, K), columns, device = scatter_map.shape, x.shape[1], x.device
-    out = torch.empty((plan_rows, columns), dtype=x.dtype, device=device)
+    out = x.new_empty((plan_rows, columns))
     xr, pitch = row_pointer(x)
     with on_device(device):
         _lib.check(_lib.load().b200moe_token_gather(xr.data_ptr(), pitch, DTYPES[x.dtype], T, K, columns, plan_rows,
                                                     row_pairs.data_ptr(), scatter_map.data_ptr(), out.data_ptr(),
-                                                    torch.cuda.current_stream(device).cuda_stream), "b200moe_token_gather")
+                                                    stream_of(device)), "b200moe_token_gather")
     return out
 
 
 def _combine(rows: torch.Tensor, weights: Optional[torch.Tensor], scatter_map: torch.Tensor) -> torch.Tensor:
     (T, K), columns, device = scatter_map.shape, rows.shape[1], rows.device
-    out = torch.empty((T, columns), dtype=rows.dtype, device=device)
+    out = rows.new_empty((T, columns))
     rr, pitch = row_pointer(rows)
     w = None if weights is None else dense(weights)
     with on_device(device):
         _lib.check(_lib.load().b200moe_token_combine(rr.data_ptr(), pitch, DTYPES[rows.dtype],
                                                      None if w is None else w.data_ptr(), T, K, columns, rows.shape[0],
                                                      scatter_map.data_ptr(), out.data_ptr(),
-                                                     torch.cuda.current_stream(device).cuda_stream),
+                                                     stream_of(device)),
                    "b200moe_token_combine")
     return out
 
@@ -135,8 +132,8 @@ def _combine(rows: torch.Tensor, weights: Optional[torch.Tensor], scatter_map: t
 def _combine_backward(grad, rows, weights, row_pairs, scatter_map, need_rows: bool, need_weights: bool):
     """``rows`` may be None where the weights' gradient is not needed."""
     (T, K), columns, device, n = scatter_map.shape, grad.shape[1], grad.device, row_pairs.shape[0]
-    grad_rows = torch.empty((n, columns), dtype=grad.dtype, device=device) if need_rows else None
-    grad_weights = torch.empty((T, K), dtype=torch.float32, device=device) if need_weights else None
+    grad_rows = grad.new_empty((n, columns)) if need_rows else None
+    grad_weights = weights.new_empty((T, K)) if need_weights else None
     gr, g_pitch = row_pointer(grad)
     rr, r_pitch = (None, 0) if rows is None else row_pointer(rows)
     w = dense(weights)
@@ -144,7 +141,7 @@ def _combine_backward(grad, rows, weights, row_pairs, scatter_map, need_rows: bo
         _lib.check(_lib.load().b200moe_token_combine_backward(
             gr.data_ptr(), g_pitch, None if rr is None else rr.data_ptr(), r_pitch, DTYPES[grad.dtype], w.data_ptr(), T, K,
             columns, n, row_pairs.data_ptr(), scatter_map.data_ptr(), None if grad_rows is None else grad_rows.data_ptr(),
-            None if grad_weights is None else grad_weights.data_ptr(), torch.cuda.current_stream(device).cuda_stream),
+            None if grad_weights is None else grad_weights.data_ptr(), stream_of(device)),
             "b200moe_token_combine_backward")
     return grad_rows, grad_weights
 
@@ -156,7 +153,7 @@ class _GatherTokens(torch.autograd.Function):
         return _gather(x, plan.rows, plan.row_pairs, plan.scatter_map)
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, grad):
         refuse_capture("gather_tokens_backward")
         return _combine(grad, None, *ctx.saved_tensors), None
@@ -170,7 +167,7 @@ class _CombineTokens(torch.autograd.Function):
         return _combine(rows, weights, plan.scatter_map)
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, grad):
         refuse_capture("combine_tokens_backward")
         rows, weights, row_pairs, scatter_map = ctx.saved_tensors
@@ -189,7 +186,6 @@ def gather_tokens(x: torch.Tensor, plan: TokenSort) -> torch.Tensor:
     return _gather(x, plan.rows, plan.row_pairs, plan.scatter_map)
 
 
-@torch.no_grad()
 def gather_tokens_backward(grad: torch.Tensor, plan: TokenSort) -> torch.Tensor:
     """Gradient [T, n] of the x of ``gather_tokens`` from that of its result; can be captured into a CUDA graph."""
     if not isinstance(plan, TokenSort):
@@ -200,7 +196,7 @@ def gather_tokens_backward(grad: torch.Tensor, plan: TokenSort) -> torch.Tensor:
 
 def _check_weights(weights, plan: TokenSort, first: torch.Tensor) -> None:
     check_tensor(weights, "topk_weights", torch.float32, tuple(plan.scatter_map.shape))
-    check_device(first, topk_weights=weights)
+    check_device(first, weights)
 
 
 def combine_tokens(rows: torch.Tensor, topk_weights: torch.Tensor, plan: TokenSort) -> torch.Tensor:
@@ -217,7 +213,6 @@ def combine_tokens(rows: torch.Tensor, topk_weights: torch.Tensor, plan: TokenSo
     return _combine(rows, topk_weights, plan.scatter_map)
 
 
-@torch.no_grad()
 def combine_tokens_backward(grad: torch.Tensor, rows: torch.Tensor, topk_weights: torch.Tensor, plan: TokenSort):
     """Gradients (grad_rows, grad_weights) of ``combine_tokens`` from that of its result, in one pass over the rows; can be
     captured into a CUDA graph."""
@@ -225,7 +220,7 @@ def combine_tokens_backward(grad: torch.Tensor, rows: torch.Tensor, topk_weights
         raise TypeError("plan must be a TokenSort")
     _check_batch(grad, "grad", plan, plan.scatter_map.shape[0])
     check_tensor(rows, "rows", grad.dtype, (plan.rows, grad.shape[1]))
-    check_device(grad, rows=rows)
+    check_device(grad, rows)
     _check_weights(topk_weights, plan, grad)
     return _combine_backward(grad, rows, topk_weights, plan.row_pairs, plan.scatter_map, True, True)
 
@@ -233,29 +228,29 @@ def combine_tokens_backward(grad: torch.Tensor, rows: torch.Tensor, topk_weights
 def _check_logits(routing_logits, topk_idx) -> tuple:
     T, K = _selection(topk_idx)
     check_tensor(routing_logits, "routing_logits", torch.float32, (T, E_GLOBAL))
-    check_device(routing_logits, topk_idx=topk_idx)
+    check_device(routing_logits, topk_idx)
     return T, K
 
 
 def _route_weights(logits, idx, scale: float) -> torch.Tensor:
     T, K = idx.shape
-    out = torch.empty((T, K), dtype=torch.float32, device=logits.device)
+    out = logits.new_empty((T, K))
     logits, idx = dense(logits), dense(idx)
     with on_device(logits.device):
         _lib.check(_lib.load().b200moe_route_weights(logits.data_ptr(), idx.data_ptr(), T, K, scale, out.data_ptr(),
-                                                     torch.cuda.current_stream(logits.device).cuda_stream),
+                                                     stream_of(logits.device)),
                    "b200moe_route_weights")
     return out
 
 
 def _route_weights_backward(logits, idx, grad, scale: float) -> torch.Tensor:
     T, K = idx.shape
-    out = torch.empty((T, E_GLOBAL), dtype=torch.float32, device=logits.device)
+    out = logits.new_empty((T, E_GLOBAL))
     logits, idx, grad = dense(logits), dense(idx), dense(grad)
     with on_device(logits.device):
         _lib.check(_lib.load().b200moe_route_weights_backward(logits.data_ptr(), idx.data_ptr(), grad.data_ptr(), T, K, scale,
                                                               out.data_ptr(),
-                                                              torch.cuda.current_stream(logits.device).cuda_stream),
+                                                              stream_of(logits.device)),
                    "b200moe_route_weights_backward")
     return out
 
@@ -268,7 +263,7 @@ class _RouteWeights(torch.autograd.Function):
         return _route_weights(logits, idx, scale)
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, grad):
         refuse_capture("route_weights_backward")
         return _route_weights_backward(*ctx.saved_tensors, grad, ctx.scale), None, None
@@ -287,11 +282,10 @@ def route_weights(routing_logits: torch.Tensor, topk_idx: torch.Tensor, routed_s
     return _route_weights(routing_logits, topk_idx, scale)
 
 
-@torch.no_grad()
 def route_weights_backward(routing_logits: torch.Tensor, topk_idx: torch.Tensor, grad_weights: torch.Tensor,
                            routed_scaling_factor) -> torch.Tensor:
     """Gradient [T, 256] of the logits of ``route_weights`` from that of its result; can be captured into a CUDA graph."""
     T, K = _check_logits(routing_logits, topk_idx)
     check_tensor(grad_weights, "grad_weights", torch.float32, (T, K))
-    check_device(routing_logits, grad_weights=grad_weights)
+    check_device(routing_logits, grad_weights)
     return _route_weights_backward(routing_logits, topk_idx, grad_weights, _host_scalar(routed_scaling_factor, float))

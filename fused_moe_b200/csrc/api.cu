@@ -220,7 +220,7 @@ static bool tokens_ok(int32_t T) { return T >= 0 && T <= (1 << 24); }
 int b200moe_add_rms_norm(const void* x, int64_t x_pitch, int32_t x_type, const void* residual, int64_t residual_pitch,
                          int32_t residual_type, const void* weight, int32_t weight_type, int32_t T, int32_t columns,
                          float eps, void* stream_out, void* y_out, void* q_out, float* scale_out, void* stream) {
-  if (!tokens_ok(T) || !type_ok(x_type) || !type_ok(weight_type)) return B200MOE_EINVAL;
+  if (!tokens_ok(T) || !type_ok(x_type) || (weight_type != x_type && weight_type != B200MOE_DTYPE_F32)) return B200MOE_EINVAL;
   if (columns < 8 || columns > B200MOE_NORM_MAX_COLUMNS || columns % 8 || (q_out && columns % QBLOCK)) return B200MOE_EINVAL;
   if (residual && residual_type != x_type && residual_type != B200MOE_DTYPE_F32) return B200MOE_EINVAL;
   if (!pitch_ok(x_pitch) || !pitch_ok(residual_pitch) || !(eps >= 0.f)) return B200MOE_EINVAL;
@@ -241,7 +241,7 @@ int b200moe_add_rms_norm_backward(const void* grad_y, int64_t grad_y_pitch, int3
                                   int32_t stream_type, const void* weight, int32_t weight_type, int32_t T, int32_t columns,
                                   float eps, void* grad_x, void* grad_residual, void* grad_weight, float* partial,
                                   void* stream) {
-  if (!tokens_ok(T) || !type_ok(type) || !type_ok(weight_type)) return B200MOE_EINVAL;
+  if (!tokens_ok(T) || !type_ok(type) || (weight_type != type && weight_type != B200MOE_DTYPE_F32)) return B200MOE_EINVAL;
   if (columns < 8 || columns > B200MOE_NORM_MAX_COLUMNS || columns % 8) return B200MOE_EINVAL;
   if (stream_type != type && stream_type != B200MOE_DTYPE_F32) return B200MOE_EINVAL;
   if (!pitch_ok(grad_y_pitch) || !pitch_ok(grad_stream_pitch) || !pitch_ok(stream_pitch) || !(eps >= 0.f))

@@ -16,191 +16,292 @@
 
 namespace b200moe {
 
-// Sum over the CTA of N values at once; `s` has 32 * N floats and is not reused before the next barrier.
-template <int N>
-__device__ __forceinline__ void block_sum(float (&v)[N], float* s) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+constexpr int MAX_WARPS = 16;   // of a CTA
+
+__device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1)
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+// Two sums over the warp for the price of little more than one: after the first exchange lanes 0..15 hold half sums of `a` and lanes
+// 16..31 of `b`.  Returns the half-warp's own sum.
+__device__ __forceinline__ float warp_sum_halves(float a, float b) {
+  const bool upper = threadIdx.x & 16;
+  float v = (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], d);
-  if (lane == 0)
-#pragma unroll
-    for (int i = 0; i < N; ++i) s[i * 32 + warp] = v[i];
+  for (int d = 8; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+// The threads of a row: a warp, or a whole number of warps with a barrier of their own (1 + group; 0 is __syncthreads).
+__device__ __forceinline__ void row_barrier(int group, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory");
+}
+// Sum over the CTA; `s` has MAX_WARPS floats and is not written again before the next barrier.
+__device__ __forceinline__ float block_sum(float v, float* s) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  v = warp_sum(v);
+  if (lane == 0) s[threadIdx.x >> 5] = v;
   __syncthreads();
+  v = lane < warps ? s[lane] : 0.f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = lane < warps ? s[i * 32 + lane] : 0.f;
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1)
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], d);
+  for (int d = MAX_WARPS / 2; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d, MAX_WARPS);
+  return __shfl_sync(0xffffffffu, v, 0);
 }
 
-// One CTA per token; a thread holds VPT vectors of eight columns, blockDim.x vectors apart, so that a half-warp holds a whole
-// 128-column block.
-template <typename X, typename R, int VPT>
-__global__ void __launch_bounds__(512)
+// Largest magnitude; a NaN where there is one.
+__device__ __forceinline__ float max_abs_nan(float m, float a) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(m), "f"(fabsf(a)));
+  return d;
+}
+
+// A row is VPT vectors of eight columns per thread, as many vectors apart as the row has threads, so that a half-warp holds a whole 128-column
+// block.  WARP_ROW: a warp per token, several tokens per CTA, and no barrier; else one CTA per token.
+template <typename X, typename R, typename W, int VPT, bool WARP_ROW>
+__global__ void __launch_bounds__(MAX_WARPS * 32)
 k_add_rms_norm(const uint8_t* x, long long x_pitch, const uint8_t* residual, long long residual_pitch,
-               const uint8_t* weight, int weight_type, int T, int n_vec, float eps, uint8_t* stream, uint8_t* y,
-               uint8_t* q, float* scale) {
-  __shared__ float s_sum[32];
-  const int t = blockIdx.x;
+               const uint8_t* weight, int T, int n_vec, float eps, uint8_t* stream, uint8_t* y, uint8_t* q, float* scale) {
+  __shared__ float s_sum[MAX_WARPS];
+  const int tid = WARP_ROW ? threadIdx.x & 31 : threadIdx.x, stride = WARP_ROW ? 32 : blockDim.x;
+  const int t = WARP_ROW ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   pdl_launch_dependents();
   pdl_wait();
+  if (WARP_ROW && t >= T) return;
+  const uint8_t* x_row = x + t * x_pitch;
+  const uint8_t* residual_row = residual + t * residual_pitch;
+  const long long row = static_cast<long long>(t) * n_vec;   // in vectors, of the dense rows
   Vec8<X> xv[VPT];
   Vec8<R> rv[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int v = threadIdx.x + i * blockDim.x;
+    const int v = tid + i * stride;
     if (v >= n_vec) continue;
-    xv[i] = load_vec8<X>(x + t * x_pitch, v);
-    if (residual) rv[i] = load_vec8<R>(residual + t * residual_pitch, v);
+    xv[i] = load_vec8<X>(x_row, v);
+    if (residual) rv[i] = load_vec8<R>(residual_row, v);
   }
-  float r[VPT][8];
-  float sum[1] = {0.f};
+  float2 r[VPT][4], sum2 = both(0.f);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int v = threadIdx.x + i * blockDim.x;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) r[i][j] = 0.f;
+    const int v = tid + i * stride;
     if (v >= n_vec) continue;
     unpack_vec8<X>(xv[i], r[i]);
     if (residual) {
-      float a[8];
+      float2 a[4];
       unpack_vec8<R>(rv[i], a);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] += r[i][j];
+      for (int j = 0; j < 4; ++j) a[j] = add2(a[j], r[i][j]);
       const Vec8<R> rounded = pack_vec8<R>(a);
-      store_vec8<R>(stream + static_cast<long long>(t) * n_vec * 8 * sizeof(R), v, rounded);
+      store_vec8<R>(stream + row * 8 * sizeof(R), v, rounded);
       unpack_vec8<R>(rounded, r[i]);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum[0] = fmaf(r[i][j], r[i][j], sum[0]);
+    for (int j = 0; j < 4; ++j) sum2 = fma2(r[i][j], r[i][j], sum2);
   }
-  block_sum(sum, s_sum);
-  const float rstd = __frsqrt_rn(sum[0] / static_cast<float>(n_vec * 8) + eps);
+  Vec8<W> wv[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int v = threadIdx.x + i * blockDim.x;
+    const int v = tid + i * stride;
+    if (v < n_vec) wv[i] = load_vec8<W>(weight, v);
+  }
+  const float sum = WARP_ROW ? warp_sum(sum2.x + sum2.y) : block_sum(sum2.x + sum2.y, s_sum);
+  const float2 rstd = both(__frsqrt_rn(sum / static_cast<float>(n_vec * 8) + eps));
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = tid + i * stride;
     if (v >= n_vec) continue;
-    float w[8];
-    load_vec8_any(weight, v, weight_type, w);
+    float2 w[4];
+    unpack_vec8<W>(wv[i], w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r[i][j] = r[i][j] * rstd * w[j];
-    if (y) store_vec8<X>(y + static_cast<long long>(t) * n_vec * 8 * sizeof(X), v, pack_vec8<X>(r[i]));
+    for (int j = 0; j < 4; ++j) r[i][j] = mul2(mul2(r[i][j], rstd), w[j]);
+    if (y) store_vec8<X>(y + row * 8 * sizeof(X), v, pack_vec8<X>(r[i]));
     if (q) {   // n_vec is a multiple of 16 here: a half-warp is inside the row or outside as a whole
-      uint32_t m = 0;
+      float m = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(r[i][j]) & 0x7fffffffu);
-      // the largest pattern is a NaN where there is one: it then stands in the scale too
-      const float amax = __uint_as_float(__reduce_max_sync((threadIdx.x & 16) ? 0xffff0000u : 0x0000ffffu, m));
+      for (int j = 0; j < 4; ++j) m = max_abs_nan(max_abs_nan(m, r[i][j].x), r[i][j].y);
+      // patterns of non-negative floats order like the floats, and a NaN (as max.NaN gives it) is above them all: it then stands in
+      // the scale too
+      const float amax =
+          __uint_as_float(__reduce_max_sync((threadIdx.x & 16) ? 0xffff0000u : 0x0000ffffu, __float_as_uint(m)));
       float s = __fmul_rn(amax, 1.0f / 448.0f);
       if (s < 1e-12f) s = 1e-12f;
       const float inv = __frcp_rn(s);
       uint2 out;
-      out.x = quantize_pair(r[i][0], r[i][1], inv) | (quantize_pair(r[i][2], r[i][3], inv) << 16);
-      out.y = quantize_pair(r[i][4], r[i][5], inv) | (quantize_pair(r[i][6], r[i][7], inv) << 16);
-      reinterpret_cast<uint2*>(q)[static_cast<long long>(t) * n_vec + v] = out;
-      if ((threadIdx.x & 15) == 0) scale[static_cast<long long>(v >> 4) * T + t] = s;
+      out.x = quantize_pair(r[i][0].x, r[i][0].y, inv) | (quantize_pair(r[i][1].x, r[i][1].y, inv) << 16);
+      out.y = quantize_pair(r[i][2].x, r[i][2].y, inv) | (quantize_pair(r[i][3].x, r[i][3].y, inv) << 16);
+      reinterpret_cast<uint2*>(q)[row + v] = out;
+      if ((tid & 15) == 0) scale[static_cast<long long>(v >> 4) * T + t] = s;
     }
   }
 }
 
-// Grid-stride over the tokens: a thread keeps its columns, so dweight accumulates in registers over the CTA's tokens and leaves
-// as one float32 row of `partial` per CTA.  Fixed order of every sum: two runs give the same bits.
-template <typename X, typename R, int VPT>
-__global__ void __launch_bounds__(512)
+// A CTA works on `groups` tokens at a time, `row_threads` threads each (narrow rows: several; wide rows: one), grid-stride over the
+// tokens.  A thread keeps its columns, so dweight accumulates in registers over the CTA's tokens; the groups' sums are added in
+// order at the end and leave as one float32 row of `partial` per CTA.  Fixed order of every sum: two runs give the same bits.
+//
+// The rows of a group's next STAGES - 1 tokens are under way in shared memory (16-byte asynchronous copies) while one is worked
+// on: a row's two passes (sums, then output) have a sum over its threads between them, in which nothing would be loaded
+// otherwise.  A thread copies exactly the pieces that it reads itself, so its own wait orders them and the pipeline needs no
+// barrier.
+template <typename X, typename R, typename W, int VPT, int STAGES, bool EXACT>
+__global__ void __launch_bounds__(MAX_WARPS * 32)
 k_add_rms_norm_backward(const uint8_t* grad_y, long long grad_y_pitch, const uint8_t* grad_stream,
                         long long grad_stream_pitch, const uint8_t* stream, long long stream_pitch, const uint8_t* weight,
-                        int weight_type, int T, int n_vec, float eps, uint8_t* grad_x, uint8_t* grad_residual,
+                        int T, int n_vec, int row_threads, float eps, uint8_t* grad_x, uint8_t* grad_residual,
                         float* partial) {
-  __shared__ float s_sum[2][64];
+  extern __shared__ uint4 s_rows[];   // [groups][STAGES][grad_y | stream | grad_stream (if given)]
+  __shared__ float s_sum[2][2][MAX_WARPS];
+  constexpr int PX = Vec8<X>::PIECES, PR = Vec8<R>::PIECES;
+  const int groups = blockDim.x / row_threads, group = threadIdx.x / row_threads;
+  const int tid = threadIdx.x - group * row_threads, lane = threadIdx.x & 31;
+  const int stage_pieces = n_vec * (PX + PR + (grad_stream ? PR : 0));
+  const uint4* rows = s_rows + group * STAGES * stage_pieces;
+  const uint32_t base = smem_u32(rows);
+  const int step = gridDim.x * groups;
   pdl_launch_dependents();
   pdl_wait();
-  float acc[VPT][8];
+  auto fetch = [&](int t, int stage) {
+    if (t < T) {
+      const uint32_t slot = base + stage * stage_pieces * 16;
+      const uint8_t* g_row = grad_y + t * grad_y_pitch;
+      const uint8_t* r_row = stream + t * stream_pitch;
+      const uint8_t* o_row = grad_stream + t * grad_stream_pitch;
 #pragma unroll
-  for (int i = 0; i < VPT; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
-  int parity = 0;
-  for (int t = blockIdx.x; t < T; t += gridDim.x, parity ^= 1) {
-    Vec8<X> gv[VPT];
-    Vec8<R> rv[VPT], ov[VPT];
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
-      if (v >= n_vec) continue;
-      gv[i] = load_vec8<X>(grad_y + t * grad_y_pitch, v);
-      rv[i] = load_vec8<R>(stream + t * stream_pitch, v);
-      if (grad_stream) ov[i] = load_vec8<R>(grad_stream + t * grad_stream_pitch, v);
-    }
-    float sum[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
-      if (v >= n_vec) continue;
-      float g[8], r[8], w[8];
-      unpack_vec8<X>(gv[i], g);
-      unpack_vec8<R>(rv[i], r);
-      load_vec8_any(weight, v, weight_type, w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        sum[0] = fmaf(r[j], r[j], sum[0]);
-        sum[1] = fmaf(g[j] * w[j], r[j], sum[1]);
+      for (int i = 0; i < VPT; ++i) {
+        const int v = tid + i * row_threads;
+        if (!EXACT && v >= n_vec) continue;
+        copy_vec8<X>(slot, g_row, v);
+        copy_vec8<R>(slot + n_vec * PX * 16, r_row, v);
+        if (grad_stream) copy_vec8<R>(slot + n_vec * (PX + PR) * 16, o_row, v);
       }
     }
-    block_sum(sum, s_sum[parity]);
-    const float n = static_cast<float>(n_vec * 8);
-    const float rstd = __frsqrt_rn(sum[0] / n + eps);
-    const float c = rstd * rstd * (sum[1] / n);
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
-      if (v >= n_vec) continue;
-      float g[8], r[8], w[8], d[8];
-      unpack_vec8<X>(gv[i], g);
-      unpack_vec8<R>(rv[i], r);
-      load_vec8_any(weight, v, weight_type, w);
-      if (grad_stream) unpack_vec8<R>(ov[i], d);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        acc[i][j] = fmaf(g[j], r[j] * rstd, acc[i][j]);
-        const float dr = rstd * (g[j] * w[j] - r[j] * c);
-        d[j] = grad_stream ? dr + d[j] : dr;
-      }
-      if (grad_x) store_vec8<X>(grad_x + static_cast<long long>(t) * n_vec * 8 * sizeof(X), v, pack_vec8<X>(d));
-      if (grad_residual)
-        store_vec8<R>(grad_residual + static_cast<long long>(t) * n_vec * 8 * sizeof(R), v, pack_vec8<R>(d));
-    }
-  }
-  if (!partial) return;
+    cp_async_commit();   // a group per token, empty behind the last
+  };
+  float2 acc[VPT][4];
+  Vec8<W> wv[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int v = threadIdx.x + i * blockDim.x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = both(0.f);
+    const int v = tid + i * row_threads;
+    if (EXACT || v < n_vec) wv[i] = load_vec8<W>(weight, v);
+  }
+  const int first = blockIdx.x * groups + group;
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) fetch(first + i * step, i);
+  int parity = 0, stage = 0;
+  for (int t = first; t < T; t += step, parity ^= 1) {
+    fetch(t + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
+    cp_async_wait_group<STAGES - 1>();
+    const uint4* slot = rows + stage * stage_pieces;
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+    float2 squares = both(0.f), mixed = both(0.f);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = tid + i * row_threads;
+      if (!EXACT && v >= n_vec) continue;
+      float2 g[4], r[4], w[4];
+      unpack_vec8<X>(shared_vec8<X>(slot, v), g);
+      unpack_vec8<R>(shared_vec8<R>(slot + n_vec * PX, v), r);
+      unpack_vec8<W>(wv[i], w);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        squares = fma2(r[j], r[j], squares);
+        mixed = fma2(mul2(g[j], r[j]), w[j], mixed);
+      }
+    }
+    float half = warp_sum_halves(squares.x + squares.y, mixed.x + mixed.y);
+    if (row_threads > 32) {
+      const int warp = threadIdx.x >> 5, row_warps = row_threads >> 5;
+      if ((lane & 15) == 0) s_sum[parity][lane >> 4][warp] = half;
+      row_barrier(group, row_threads);
+      half = (lane & 15) < row_warps ? s_sum[parity][lane >> 4][group * row_warps + (lane & 15)] : 0.f;
+#pragma unroll
+      for (int d = 8; d > 0; d >>= 1) half += __shfl_xor_sync(0xffffffffu, half, d);
+    }
+    const float n = static_cast<float>(n_vec * 8);
+    const float rstd1 = __frsqrt_rn(__shfl_sync(0xffffffffu, half, 0) / n + eps);
+    const float mean = __shfl_sync(0xffffffffu, half, 16) / n;
+    const float2 rstd = both(rstd1), c = both(-(rstd1 * rstd1 * rstd1 * mean));
+    const long long row = static_cast<long long>(t) * n_vec;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = tid + i * row_threads;
+      if (!EXACT && v >= n_vec) continue;
+      float2 g[4], r[4], w[4], d[4];
+      unpack_vec8<X>(shared_vec8<X>(slot, v), g);
+      unpack_vec8<R>(shared_vec8<R>(slot + n_vec * PX, v), r);
+      unpack_vec8<W>(wv[i], w);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[j] = both(0.f);
+      if (grad_stream) unpack_vec8<R>(shared_vec8<R>(slot + n_vec * (PX + PR), v), d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        g[j] = mul2(g[j], rstd);
+        acc[i][j] = fma2(g[j], r[j], acc[i][j]);
+        d[j] = fma2(g[j], w[j], fma2(r[j], c, d[j]));
+      }
+      if (grad_x) store_vec8<X>(grad_x + row * 8 * sizeof(X), v, pack_vec8<X>(d));
+      if (grad_residual) store_vec8<R>(grad_residual + row * 8 * sizeof(R), v, pack_vec8<R>(d));
+    }
+  }
+  cp_async_wait_group<0>();
+  if (!partial) return;
+  if (groups > 1) {   // the rows' space is free behind the barrier: it holds the sums of groups 1, 2, ... (checked by the host)
+    __syncthreads();
+    uint8_t* sums = reinterpret_cast<uint8_t*>(s_rows);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = tid + i * row_threads;
+      if (group > 0 && v < n_vec) store_vec8<float>(sums, (group - 1) * n_vec + v, pack_vec8<float>(acc[i]));
+    }
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int v = tid + i * row_threads;
+      if (v >= n_vec) continue;
+      for (int k = 1; k < groups; ++k) {
+        float2 more[4];
+        unpack_vec8<float>(shared_vec8<float>(s_rows, (k - 1) * n_vec + v), more);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = add2(acc[i][j], more[j]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int v = tid + i * row_threads;
     if (v < n_vec)
       store_vec8<float>(reinterpret_cast<uint8_t*>(partial + static_cast<long long>(blockIdx.x) * n_vec * 8), v,
                         pack_vec8<float>(acc[i]));
   }
 }
 
-// dweight[c] = sum of the rows of `partial`, rounded once: 32 columns per CTA, eight warps a row each in turn.
-__global__ void __launch_bounds__(256)
+// dweight[c] = sum of the rows of `partial`, rounded once: 32 columns per CTA, its warps take the rows in turn, sixteen in flight.
+constexpr int WEIGHT_GRAD_WARPS = 16;
+__global__ void __launch_bounds__(WEIGHT_GRAD_WARPS * 32)
 k_norm_weight_grad(const float* partial, int rows, int columns, int type, void* grad_weight) {
-  __shared__ float s[8][32];
+  __shared__ float s[WEIGHT_GRAD_WARPS][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   pdl_launch_dependents();
   pdl_wait();
   float sum = 0.f;
-  if (c < columns) {
-#pragma unroll 8
-    for (int r = warp; r < rows; r += 8) sum += ld_dep(partial + static_cast<long long>(r) * columns + c);
+  for (int r = warp; c < columns && r < rows; r += 16 * WEIGHT_GRAD_WARPS) {
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int row = r + i * WEIGHT_GRAD_WARPS;
+      v[i] = row < rows ? ld_dep(partial + static_cast<long long>(row) * columns + c) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += v[i];
   }
   s[warp][lane] = sum;
   __syncthreads();
   if (warp != 0 || c >= columns) return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) sum += s[i][lane];
+  for (int i = 1; i < WEIGHT_GRAD_WARPS; ++i) sum += s[i][lane];
   if (type == B200MOE_DTYPE_F32) {
     static_cast<float*>(grad_weight)[c] = sum;
   } else if (type == B200MOE_DTYPE_F16) {
@@ -210,41 +311,65 @@ k_norm_weight_grad(const float* partial, int rows, int columns, int type, void* 
   }
 }
 
+constexpr size_t MAX_DYNAMIC_SMEM = 227 * 1024 - 1024;   // of a CTA, less the static arrays
+
+// Vectors of eight columns per thread.  Forward: few tokens want many threads each (a CTA's latency is the call's), many tokens
+// few and fat ones (the row's sum costs per warp).  us at 7168 columns, two / four vectors: 1 token 2.3 / 2.8, 333 tokens
+// 4.2 / 5.0, 1500 tokens 11.7 / 11.8, 16384 tokens 130 / 125 (e4m3 out), 8192 tokens without a residual 46 / 40.
+static int forward_vpt(int T, int n_vec) { return n_vec > 1024 || (n_vec > 64 && T > 1024) ? 4 : n_vec > 32 ? 2 : 1; }
+// Backward: four where they leave two CTAs per SM (16-bit rows), us at 8192 x 7168 with two / four: bf16 86 / 79, bf16 with a
+// float32 stream 143 / 158; bf16 at 2048 columns 29 / 31.
+static int backward_vpt(bool wide_stream, int n_vec) {
+  return n_vec > 1024 || (n_vec > 512 && !wide_stream) ? 4 : n_vec > 32 ? 2 : 1;
+}
+constexpr int BACKWARD_THREADS = 256;   // of a CTA that works on several tokens at once
 struct NormShape {
-  int n_vec, vpt, threads;
+  int n_vec, vpt, threads;   // threads: of a row
 };
-static NormShape norm_shape(int columns) {
+static NormShape norm_shape(int columns, int vpt) {
   NormShape s;
   s.n_vec = columns / 8;
-  s.vpt = s.n_vec > 512 ? 4 : s.n_vec > 256 ? 2 : 1;
-  s.threads = ((s.n_vec + s.vpt - 1) / s.vpt + 31) / 32 * 32;
+  s.vpt = vpt;
+  s.threads = ((s.n_vec + vpt - 1) / vpt + 31) / 32 * 32;
   return s;
 }
 
-// Calls f with (X tag, R tag, VPT) of the given types; the residual stream has x's type or float32.
-template <typename X, typename R, typename F>
+// Calls f with tags of the types and VPT.  The residual stream and the weight have x's type or float32.
+template <typename X, typename R, typename W, typename F>
 static int with_vpt(int vpt, F&& f) {
-  if (vpt == 4) return f(X(), R(), std::integral_constant<int, 4>());
-  if (vpt == 2) return f(X(), R(), std::integral_constant<int, 2>());
-  return f(X(), R(), std::integral_constant<int, 1>());
+  if (vpt == 4) return f(X(), R(), W(), std::integral_constant<int, 4>());
+  if (vpt == 2) return f(X(), R(), W(), std::integral_constant<int, 2>());
+  return f(X(), R(), W(), std::integral_constant<int, 1>());
+}
+template <typename X, typename F>
+static int with_16_bit(bool wide_stream, bool wide_weight, int vpt, F&& f) {
+  if (wide_stream) return wide_weight ? with_vpt<X, float, float>(vpt, f) : with_vpt<X, float, X>(vpt, f);
+  return wide_weight ? with_vpt<X, X, float>(vpt, f) : with_vpt<X, X, X>(vpt, f);
 }
 template <typename F>
-static int with_types(int x_type, int stream_type, int vpt, F&& f) {
-  if (x_type == B200MOE_DTYPE_F32) return with_vpt<float, float>(vpt, f);
-  if (x_type == B200MOE_DTYPE_F16)
-    return stream_type == x_type ? with_vpt<__half, __half>(vpt, f) : with_vpt<__half, float>(vpt, f);
-  return stream_type == x_type ? with_vpt<__nv_bfloat16, __nv_bfloat16>(vpt, f) : with_vpt<__nv_bfloat16, float>(vpt, f);
+static int with_types(int x_type, int stream_type, int weight_type, int vpt, F&& f) {
+  const bool wide_stream = stream_type == B200MOE_DTYPE_F32, wide_weight = weight_type == B200MOE_DTYPE_F32;
+  if (x_type == B200MOE_DTYPE_F32) return with_vpt<float, float, float>(vpt, f);
+  if (x_type == B200MOE_DTYPE_F16) return with_16_bit<__half>(wide_stream, wide_weight, vpt, f);
+  return with_16_bit<__nv_bfloat16>(wide_stream, wide_weight, vpt, f);
 }
 
 int launch_add_rms_norm(const void* x, long long x_pitch, int x_type, const void* residual, long long residual_pitch,
                         int residual_type, const void* weight, int weight_type, int T, int columns, float eps,
                         void* stream_out, void* y, void* q, float* scale, int num_sms, cudaStream_t st) {
-  const NormShape s = norm_shape(columns);
-  return with_types(x_type, residual ? residual_type : x_type, s.vpt, [&](auto xt, auto rt, auto vpt) -> int {
-    auto kern = k_add_rms_norm<decltype(xt), decltype(rt), decltype(vpt)::value>;
-    B200MOE_CUDA_TRY(launch_pdl(kern, dim3(T), dim3(s.threads), 0, st, static_cast<const uint8_t*>(x), x_pitch,
-                                static_cast<const uint8_t*>(residual), residual_pitch,
-                                static_cast<const uint8_t*>(weight), weight_type, T, s.n_vec, eps,
+  const NormShape s = norm_shape(columns, forward_vpt(T, columns / 8));
+  return with_types(x_type, residual ? residual_type : x_type, weight_type, s.vpt,
+                    [&](auto xt, auto rt, auto wt, auto vpt) -> int {
+    using X = decltype(xt);
+    using R = decltype(rt);
+    using W = decltype(wt);
+    constexpr int VPT = decltype(vpt)::value;
+    constexpr int ROWS = 4;   // of a CTA where a warp has a row to itself
+    const bool warp_row = s.threads == 32;
+    auto kern = warp_row ? k_add_rms_norm<X, R, W, VPT, true> : k_add_rms_norm<X, R, W, VPT, false>;
+    B200MOE_CUDA_TRY(launch_pdl(kern, dim3(warp_row ? (T + ROWS - 1) / ROWS : T), dim3(warp_row ? 32 * ROWS : s.threads), 0,
+                                st, static_cast<const uint8_t*>(x), x_pitch, static_cast<const uint8_t*>(residual),
+                                residual_pitch, static_cast<const uint8_t*>(weight), T, s.n_vec, eps,
                                 static_cast<uint8_t*>(stream_out), static_cast<uint8_t*>(y), static_cast<uint8_t*>(q),
                                 scale));
     return B200MOE_OK;
@@ -255,20 +380,43 @@ int launch_add_rms_norm_backward(const void* grad_y, long long grad_y_pitch, int
                                  long long grad_stream_pitch, const void* stream, long long stream_pitch, int stream_type,
                                  const void* weight, int weight_type, int T, int columns, float eps, void* grad_x,
                                  void* grad_residual, void* grad_weight, float* partial, int num_sms, cudaStream_t st) {
-  const NormShape s = norm_shape(columns);
-  int ctas = T < B200MOE_NORM_PARTIAL_ROWS ? T : B200MOE_NORM_PARTIAL_ROWS;
-  if (ctas > 2 * num_sms) ctas = 2 * num_sms;
-  const int rc = with_types(type, stream_type, s.vpt, [&](auto xt, auto rt, auto vpt) -> int {
-    auto kern = k_add_rms_norm_backward<decltype(xt), decltype(rt), decltype(vpt)::value>;
-    B200MOE_CUDA_TRY(launch_pdl(kern, dim3(ctas), dim3(s.threads), 0, st, static_cast<const uint8_t*>(grad_y),
-                                grad_y_pitch, static_cast<const uint8_t*>(grad_stream), grad_stream_pitch,
-                                static_cast<const uint8_t*>(stream), stream_pitch, static_cast<const uint8_t*>(weight),
-                                weight_type, T, s.n_vec, eps, static_cast<uint8_t*>(grad_x),
-                                static_cast<uint8_t*>(grad_residual), grad_weight ? partial : nullptr));
-    return B200MOE_OK;
+  const NormShape s = norm_shape(columns, backward_vpt(stream_type == B200MOE_DTYPE_F32, columns / 8));
+  int ctas = 0;
+  const int rc = with_types(type, stream_type, weight_type, s.vpt, [&](auto xt, auto rt, auto wt, auto vpt) -> int {
+    using X = decltype(xt);
+    using R = decltype(rt);
+    using W = decltype(wt);
+    constexpr int VPT = decltype(vpt)::value;
+    const size_t stage = static_cast<size_t>(columns) * (sizeof(X) + sizeof(R) * (grad_stream ? 2 : 1));
+    // tokens that a CTA works on at once: about BACKWARD_THREADS threads' worth
+    const int groups = s.threads >= BACKWARD_THREADS ? 1 : BACKWARD_THREADS / s.threads;
+    auto launch = [&](auto kern, int stages) -> int {
+      const size_t smem = stage * stages * groups;
+      static_assert(sizeof(X) + sizeof(R) >= 4, "two stages of a row hold its columns in float32: the groups' sums fit");
+      B200MOE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+      int per_sm = 0;
+      B200MOE_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, s.threads * groups, smem));
+      int most = num_sms * (per_sm > 0 ? per_sm : 1);
+      if (most > B200MOE_NORM_PARTIAL_ROWS) most = B200MOE_NORM_PARTIAL_ROWS;
+      const int batches = (T + groups - 1) / groups;
+      const int rounds = (batches + most - 1) / most;   // of the busiest CTA; no more CTAs than that takes
+      ctas = (batches + rounds - 1) / rounds;
+      B200MOE_CUDA_TRY(launch_pdl(kern, dim3(ctas), dim3(s.threads * groups), smem, st, static_cast<const uint8_t*>(grad_y),
+                                  grad_y_pitch, static_cast<const uint8_t*>(grad_stream), grad_stream_pitch,
+                                  static_cast<const uint8_t*>(stream), stream_pitch,
+                                  static_cast<const uint8_t*>(weight), T, s.n_vec, s.threads, eps,
+                                  static_cast<uint8_t*>(grad_x), static_cast<uint8_t*>(grad_residual),
+                                  grad_weight ? partial : nullptr));
+      return B200MOE_OK;
+    };
+    const bool exact = s.n_vec == VPT * s.threads;
+    if (2 * stage * groups <= MAX_DYNAMIC_SMEM)
+      return exact ? launch(k_add_rms_norm_backward<X, R, W, VPT, 2, true>, 2)
+                   : launch(k_add_rms_norm_backward<X, R, W, VPT, 2, false>, 2);
+    return launch(k_add_rms_norm_backward<X, R, W, VPT, 1, false>, 1);
   });
   if (rc || !grad_weight) return rc;
-  B200MOE_CUDA_TRY(launch_pdl(k_norm_weight_grad, dim3((columns + 31) / 32), dim3(256), 0, st,
+  B200MOE_CUDA_TRY(launch_pdl(k_norm_weight_grad, dim3((columns + 31) / 32), dim3(WEIGHT_GRAD_WARPS * 32), 0, st,
                               static_cast<const float*>(partial), ctas, columns, weight_type, grad_weight));
   return B200MOE_OK;
 }

@@ -199,7 +199,7 @@ k_token_combine(const uint8_t* in, long long in_pitch, const float* weights, int
                 const int* scatter_map, uint8_t* out) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int N = PIECE_ELEMS<X>;
+  constexpr int N = PIECE_PAIRS<X>;
   const int t = blockIdx.x;
   int row[TOP_K];
   float w[TOP_K];
@@ -211,16 +211,16 @@ k_token_combine(const uint8_t* in, long long in_pitch, const float* weights, int
 #pragma unroll
     for (int k = 0; k < TOP_K; ++k)
       if (row[k] >= 0) raw[k] = ld_dep(reinterpret_cast<const uint4*>(in + row[k] * in_pitch) + p);
-    float acc[N];
+    float2 acc[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] = 0.f;
+    for (int j = 0; j < N; ++j) acc[j] = both(0.f);
 #pragma unroll
     for (int k = 0; k < TOP_K; ++k) {
       if (row[k] < 0) continue;
-      float f[N];
+      float2 f[N];
       unpack_piece<X>(raw[k], f);
 #pragma unroll
-      for (int j = 0; j < N; ++j) acc[j] = fmaf(w[k], f[j], acc[j]);
+      for (int j = 0; j < N; ++j) acc[j] = fma2(both(w[k]), f[j], acc[j]);
     }
     reinterpret_cast<uint4*>(out)[static_cast<long long>(t) * pieces + p] = pack_piece<X>(acc);
   }
@@ -235,16 +235,17 @@ k_token_combine_backward(const uint8_t* grad, long long grad_pitch, const uint8_
   __shared__ float s_dot[TOP_K][8];
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int N = PIECE_ELEMS<X>;
+  constexpr int N = PIECE_PAIRS<X>;
   const int t = blockIdx.x;
   if (t < T) {
     int row[TOP_K];
-    float w[TOP_K], dot[TOP_K];
+    float w[TOP_K];
+    float2 dot2[TOP_K];
     token_rows(scatter_map, t, K, rows, row);
 #pragma unroll
     for (int k = 0; k < TOP_K; ++k) {
       w[k] = k < K ? ld_dep(weights + static_cast<long long>(t) * K + k) : 0.f;
-      dot[k] = 0.f;
+      dot2[k] = both(0.f);
     }
     for (int p = threadIdx.x; p < pieces; p += blockDim.x) {
       const uint4 raw_g = ld_dep(reinterpret_cast<const uint4*>(grad + t * grad_pitch) + p);
@@ -252,26 +253,29 @@ k_token_combine_backward(const uint8_t* grad, long long grad_pitch, const uint8_
 #pragma unroll
       for (int k = 0; k < TOP_K; ++k)
         if (grad_w && row[k] >= 0) raw[k] = ld_dep(reinterpret_cast<const uint4*>(in + row[k] * in_pitch) + p);
-      float g[N];
+      float2 g[N];
       unpack_piece<X>(raw_g, g);
 #pragma unroll
       for (int k = 0; k < TOP_K; ++k) {
         if (row[k] < 0) continue;
         if (grad_w) {
-          float f[N];
+          float2 f[N];
           unpack_piece<X>(raw[k], f);
 #pragma unroll
-          for (int j = 0; j < N; ++j) dot[k] = fmaf(g[j], f[j], dot[k]);
+          for (int j = 0; j < N; ++j) dot2[k] = fma2(g[j], f[j], dot2[k]);
         }
         if (grad_in) {
-          float d[N];
+          float2 d[N];
 #pragma unroll
-          for (int j = 0; j < N; ++j) d[j] = w[k] * g[j];
+          for (int j = 0; j < N; ++j) d[j] = mul2(both(w[k]), g[j]);
           reinterpret_cast<uint4*>(grad_in)[static_cast<long long>(row[k]) * pieces + p] = pack_piece<X>(d);
         }
       }
     }
     if (grad_w) {
+      float dot[TOP_K];
+#pragma unroll
+      for (int k = 0; k < TOP_K; ++k) dot[k] = dot2[k].x + dot2[k].y;
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1)
 #pragma unroll

@@ -30,8 +30,8 @@ def _check(x, residual, weight, eps, multiple: int, names=("x", "residual")) -> 
         if torch.is_tensor(residual) and residual.dtype is not x.dtype and residual.dtype is not torch.float32:
             raise TypeError(f"{names[1]} must have the type of {names[0]} or float32, got {residual.dtype}")
         check_tensor(residual, names[1], residual.dtype if torch.is_tensor(residual) else x.dtype, (T, columns))
-    if not torch.is_tensor(weight) or weight.dtype not in DTYPES:
-        raise TypeError("weight must be a bfloat16, float16 or float32 tensor")
+    if not torch.is_tensor(weight) or (weight.dtype is not x.dtype and weight.dtype is not torch.float32):
+        raise TypeError(f"weight must be a tensor of the type of {names[0]} or float32")
     check_tensor(weight, "weight", weight.dtype, (columns,))
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
@@ -116,8 +116,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
     """(y, r): the normalised rows in the type of ``x`` and the residual stream after the addition in the type of ``residual``.
     ``residual=None`` is the first norm of a model: r is then ``x`` itself.
 
-    x [T, n] bf16, f16 or f32, n a multiple of 8 up to 16384 · residual [T, n] of x's type or f32 · weight [n] of any of the three
-    types.  Row-strided inputs are read in place.  Differentiable once in x, residual and weight; the backward pass saves r and
+    x [T, n] bf16, f16 or f32, n a multiple of 8 up to 16384 · residual [T, n] and weight [n] each of x's type or
+    f32.  Row-strided inputs are read in place.  Differentiable once in x, residual and weight; the backward pass saves r and
     the weight only, and its sums have a fixed order.  During stream capture a call that would record a gradient is
     refused (``add_rms_norm_backward`` is the explicit form)."""
     T, columns = _check(x, residual, weight, eps, 8)

@@ -213,8 +213,8 @@ int b200moe_quantize_act(const void* x_bf16, int32_t T, void* q_out, float* scal
  * stream_out [T, columns] of residual_type receives r (it may be `residual` itself); y_out (optional) y in x_type; q_out and
  * scale_out (optional, together) e4m3 rows and their float32 scales [columns / 128, T] by the rule of b200moe_quantize_act,
  * applied to the float32 y; a NaN in a block makes its scale NaN.
- * columns: a multiple of 8 (of 128 with q_out), at most B200MOE_NORM_MAX_COLUMNS; residual_type: x_type or float32;
- * weight [columns] of any type. */
+ * columns: a multiple of 8 (of 128 with q_out), at most B200MOE_NORM_MAX_COLUMNS; residual_type and
+ * weight_type: x_type or float32. */
 int b200moe_add_rms_norm(const void* x, int64_t x_pitch, int32_t x_type, const void* residual, int64_t residual_pitch,
                          int32_t residual_type, const void* weight, int32_t weight_type, int32_t T, int32_t columns,
                          float eps, void* stream_out, void* y_out, void* q_out, float* scale_out, void* stream);

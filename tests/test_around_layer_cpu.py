@@ -26,6 +26,7 @@ NORM_REFUSED = [
     (TypeError, dict(residual=1.0)),
     (TypeError, dict(weight=None)),
     (TypeError, dict(weight=torch.zeros(256, dtype=torch.int32))),
+    (TypeError, dict(weight=torch.zeros(256, dtype=F16))),
     (ValueError, dict(weight=torch.zeros(128))),
     (ValueError, dict(eps=-1e-6)),
     (ValueError, dict(eps=float("nan"))),
@@ -188,7 +189,7 @@ def test_norm_abi_refuses(lib):
     base = dict(x=A, x_pitch=0, x_type=0, residual=A, r_pitch=0, r_type=0, weight=A, w_type=0, T=4, columns=256, eps=1e-6,
                 stream_out=A, y=A, q=A, scale=A, stream=None)
     for change in (dict(x=None), dict(x=A + 8), dict(x_pitch=8), dict(x_pitch=-16), dict(x_type=3), dict(x_type=-1),
-                   dict(r_type=1), dict(residual=A + 2), dict(weight=None), dict(weight=A + 4), dict(w_type=7), dict(T=-1),
+                   dict(r_type=1), dict(residual=A + 2), dict(weight=None), dict(weight=A + 4), dict(w_type=7), dict(w_type=1), dict(T=-1),
                    dict(T=(1 << 24) + 1), dict(columns=0), dict(columns=260), dict(columns=264), dict(columns=16512),
                    dict(eps=-1.0), dict(eps=float("nan")), dict(stream_out=None), dict(q=None), dict(scale=None),
                    dict(y=None, q=None, scale=None), dict(y=A + 1), dict(q=A + 8)):

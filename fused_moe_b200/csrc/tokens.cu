@@ -147,151 +147,219 @@ k_token_place(const int* topk_idx, long long n_pairs, long long per, int offset,
   }
 }
 
-// The rows of token t's pairs; an entry outside 0 .. rows - 1 is none (-1), so that a map of another batch cannot lead a store
-// out of the buffer.
-__device__ __forceinline__ bool token_rows(const int* scatter_map, long long t, int K, int rows, int (&row)[TOP_K]) {
-  bool any = false;
-#pragma unroll
-  for (int k = 0; k < TOP_K; ++k) {
-    row[k] = k < K ? ld_dep(scatter_map + t * K + k) : -1;
-    if (static_cast<uint32_t>(row[k]) >= static_cast<uint32_t>(rows)) row[k] = -1;
-    any |= row[k] >= 0;
-  }
-  return any;
+// A token's pairs, one per lane of every warp: lane k < K holds the row (-1: none; an entry outside 0 .. rows - 1 is none, so that
+// a map of another batch cannot lead a store out of the buffer) and the weight of pair (t, k).  `mask`: the lanes with a row.
+struct TokenPairs {
+  int row;
+  float weight;
+  uint32_t mask;
+};
+__device__ __forceinline__ TokenPairs token_pairs(const int* scatter_map, const float* weights, long long t, int K, int rows) {
+  const int lane = threadIdx.x & 31;
+  TokenPairs p;
+  p.row = lane < K ? ld_dep(scatter_map + t * K + lane) : -1;
+  p.weight = lane < K && weights ? ld_dep(weights + t * K + lane) : 1.f;
+  if (static_cast<uint32_t>(p.row) >= static_cast<uint32_t>(rows)) p.row = -1;
+  p.mask = __ballot_sync(0xffffffffu, p.row >= 0);
+  return p;
 }
 
-// CTA i's share of the rows is looked through for rows without a pair, which become zeros.
-__device__ __forceinline__ void zero_unused_rows(const int* row_pairs, int rows, uint8_t* out, int pieces) {
-  const int begin = static_cast<int>(static_cast<long long>(rows) * blockIdx.x / gridDim.x);
-  const int end = static_cast<int>(static_cast<long long>(rows) * (blockIdx.x + 1) / gridDim.x);
-  for (int r = begin; r < end; ++r) {
-    if (ld_dep(row_pairs + r) >= 0) continue;
-    uint4* dst = reinterpret_cast<uint4*>(out) + static_cast<long long>(r) * pieces;
-    for (int p = threadIdx.x; p < pieces; p += blockDim.x) dst[p] = make_uint4(0u, 0u, 0u, 0u);
+// CTA i's share of the rows (grid.x CTAs; at most 32 rows each, checked by the host) is looked through for rows without a pair,
+// which become zeros in the pieces [begin, end) of this CTA.
+__device__ __forceinline__ void zero_unused_rows(const int* row_pairs, int rows, uint8_t* out, int pieces, int begin, int end) {
+  const int lane = threadIdx.x & 31;
+  const int first = static_cast<int>(static_cast<long long>(rows) * blockIdx.x / gridDim.x);
+  const int last = static_cast<int>(static_cast<long long>(rows) * (blockIdx.x + 1) / gridDim.x);
+  uint32_t unused = __ballot_sync(0xffffffffu, first + lane < last && ld_dep(row_pairs + min(first + lane, rows - 1)) < 0);
+  for (; unused; unused &= unused - 1) {
+    uint4* dst = reinterpret_cast<uint4*>(out) + static_cast<long long>(first + __ffs(unused) - 1) * pieces;
+    for (int p = begin + threadIdx.x; p < end; p += blockDim.x) dst[p] = make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
-// out[row(t,k)] = x[t]; one CTA per token, which also zeroes its share of the unused rows.
+// out[row(t,k)] = x[t]; CTA (t, y) copies the y-th part of the token's row, and zeroes its share of the unused rows.
+constexpr int TOKEN_UNROLL = 4;   // pieces of a row in flight per thread
 __global__ void __launch_bounds__(256)
 k_token_gather(const uint8_t* x, long long x_pitch, int T, int K, int rows, int pieces, const int* row_pairs,
                const int* scatter_map, uint8_t* out) {
   pdl_launch_dependents();
   pdl_wait();
   const int t = blockIdx.x;
+  const int part = (pieces + gridDim.y - 1) / gridDim.y, begin = blockIdx.y * part, end = min(begin + part, pieces);
   if (t < T) {
-    int row[TOP_K];
-    const bool any = token_rows(scatter_map, t, K, rows, row);
+    const TokenPairs pairs = token_pairs(scatter_map, nullptr, t, K, rows);
     const uint4* src = reinterpret_cast<const uint4*>(x + t * x_pitch);
-    for (int p = threadIdx.x; any && p < pieces; p += blockDim.x) {
-      const uint4 v = ld_dep(src + p);
+    for (int p0 = begin + threadIdx.x; pairs.mask && p0 - static_cast<int>(threadIdx.x) < end; p0 += TOKEN_UNROLL * blockDim.x) {
+      uint4 v[TOKEN_UNROLL];
 #pragma unroll
-      for (int k = 0; k < TOP_K; ++k)
-        if (row[k] >= 0) reinterpret_cast<uint4*>(out)[static_cast<long long>(row[k]) * pieces + p] = v;
+      for (int i = 0; i < TOKEN_UNROLL; ++i)
+        if (p0 + i * blockDim.x < end) v[i] = ld_dep(src + p0 + i * blockDim.x);
+      for (uint32_t m = pairs.mask; m; m &= m - 1) {
+        const int row = __shfl_sync(0xffffffffu, pairs.row, __ffs(m) - 1);
+        uint4* dst = reinterpret_cast<uint4*>(out) + static_cast<long long>(row) * pieces;
+#pragma unroll
+        for (int i = 0; i < TOKEN_UNROLL; ++i)
+          if (p0 + i * blockDim.x < end) __stcs(dst + p0 + i * blockDim.x, v[i]);
+      }
     }
   }
-  zero_unused_rows(row_pairs, rows, out, pieces);
+  zero_unused_rows(row_pairs, rows, out, pieces, begin, end);
 }
 
-// out[t] = sum_k w[t,k] * in[row(t,k)], k ascending (weights == nullptr: 1); one CTA per token.
+// The rows of up to N pairs of a token, in the order of k: the lowest N bits of the mask.
+template <int N>
+__device__ __forceinline__ void take_pairs(const TokenPairs& pairs, int (&row)[N], float (&w)[N]) {
+  uint32_t m = pairs.mask;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int k = m ? __ffs(m) - 1 : 0;
+    const int r = __shfl_sync(0xffffffffu, pairs.row, k);
+    w[j] = __shfl_sync(0xffffffffu, pairs.weight, k);
+    row[j] = m ? r : -1;
+    m &= m - 1;
+  }
+}
+
+// out[t] = sum_k w[t,k] * in[row(t,k)], k ascending (weights == nullptr: 1), over the pieces [begin, end) of the rows.  N: most
+// rows of the token; U: pieces of each in flight per thread (a token with one or two rows would have too few bytes under way
+// otherwise: a shard of 32 experts at 14107 tokens 94 us with one piece, 69 with two).  Five CTAs of 256 threads per SM.
+template <typename X, int N, int U>
+__device__ __forceinline__ void combine_rows(const uint8_t* in, long long in_pitch, const TokenPairs& pairs, int begin,
+                                             int end, uint4* out) {
+  constexpr int P = PIECE_PAIRS<X>;
+  int row[N];
+  float w[N];
+  take_pairs(pairs, row, w);
+  for (int p0 = begin + threadIdx.x; p0 < end; p0 += U * blockDim.x) {
+    uint4 raw[U][N];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (row[k] >= 0 && p0 + i * blockDim.x < end)
+          raw[i][k] = ld_dep(reinterpret_cast<const uint4*>(in + row[k] * in_pitch) + p0 + i * blockDim.x);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (p0 + i * blockDim.x >= end) break;
+      float2 acc[P];
+#pragma unroll
+      for (int j = 0; j < P; ++j) acc[j] = both(0.f);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        if (row[k] < 0) continue;
+        float2 f[P];
+        unpack_piece<X>(raw[i][k], f);
+#pragma unroll
+        for (int j = 0; j < P; ++j) acc[j] = fma2(both(w[k]), f[j], acc[j]);
+      }
+      out[p0 + i * blockDim.x] = pack_piece<X>(acc);
+    }
+  }
+}
 template <typename X>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 5)
 k_token_combine(const uint8_t* in, long long in_pitch, const float* weights, int K, int rows, int pieces,
                 const int* scatter_map, uint8_t* out) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int N = PIECE_PAIRS<X>;
   const int t = blockIdx.x;
-  int row[TOP_K];
-  float w[TOP_K];
-  token_rows(scatter_map, t, K, rows, row);
-#pragma unroll
-  for (int k = 0; k < TOP_K; ++k) w[k] = k < K && weights ? ld_dep(weights + static_cast<long long>(t) * K + k) : 1.f;
-  for (int p = threadIdx.x; p < pieces; p += blockDim.x) {
-    uint4 raw[TOP_K];
-#pragma unroll
-    for (int k = 0; k < TOP_K; ++k)
-      if (row[k] >= 0) raw[k] = ld_dep(reinterpret_cast<const uint4*>(in + row[k] * in_pitch) + p);
-    float2 acc[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] = both(0.f);
-#pragma unroll
-    for (int k = 0; k < TOP_K; ++k) {
-      if (row[k] < 0) continue;
-      float2 f[N];
-      unpack_piece<X>(raw[k], f);
-#pragma unroll
-      for (int j = 0; j < N; ++j) acc[j] = fma2(both(w[k]), f[j], acc[j]);
-    }
-    reinterpret_cast<uint4*>(out)[static_cast<long long>(t) * pieces + p] = pack_piece<X>(acc);
-  }
+  const int part = (pieces + gridDim.y - 1) / gridDim.y, begin = blockIdx.y * part, end = min(begin + part, pieces);
+  const TokenPairs pairs = token_pairs(scatter_map, weights, t, K, rows);
+  uint4* dst = reinterpret_cast<uint4*>(out) + static_cast<long long>(t) * pieces;
+  if (__popc(pairs.mask) <= 2)
+    combine_rows<X, 2, 2>(in, in_pitch, pairs, begin, end, dst);
+  else
+    combine_rows<X, TOP_K, 1>(in, in_pitch, pairs, begin, end, dst);
 }
 
-// grad_in[row(t,k)] = w[t,k] * grad[t] and grad_w[t,k] = <grad[t], in[row(t,k)]> in one pass; either output may be absent.
-template <typename X>
-__global__ void __launch_bounds__(256)
-k_token_combine_backward(const uint8_t* grad, long long grad_pitch, const uint8_t* in, long long in_pitch,
-                         const float* weights, int T, int K, int rows, int pieces, const int* row_pairs,
-                         const int* scatter_map, uint8_t* grad_in, float* grad_w) {
-  __shared__ float s_dot[TOP_K][8];
-  pdl_launch_dependents();
-  pdl_wait();
-  constexpr int N = PIECE_PAIRS<X>;
-  const int t = blockIdx.x;
-  if (t < T) {
-    int row[TOP_K];
-    float w[TOP_K];
-    float2 dot2[TOP_K];
-    token_rows(scatter_map, t, K, rows, row);
+// grad_in[row(t,k)] = w[t,k] * grad[t] and the token's dot products <grad[t], in[row(t,k)]>, summed over the CTA into
+// s_dot[j][warp] for the j-th pair with a row; N and U as for combine_rows.
+template <typename X, int N, int U>
+__device__ __forceinline__ void combine_rows_backward(const uint4* grad, const uint8_t* in, long long in_pitch,
+                                                      const TokenPairs& pairs, int pieces, uint8_t* grad_in,
+                                                      float (*s_dot)[16]) {
+  constexpr int P = PIECE_PAIRS<X>;
+  int row[N];
+  float w[N];
+  float2 dot2[N];
+  take_pairs(pairs, row, w);
 #pragma unroll
-    for (int k = 0; k < TOP_K; ++k) {
-      w[k] = k < K ? ld_dep(weights + static_cast<long long>(t) * K + k) : 0.f;
-      dot2[k] = both(0.f);
+  for (int k = 0; k < N; ++k) dot2[k] = both(0.f);
+  for (int p0 = threadIdx.x; p0 < pieces; p0 += U * blockDim.x) {
+    uint4 raw_g[U], raw[U][N];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int p = p0 + i * blockDim.x;
+      if (p >= pieces) break;
+      raw_g[i] = ld_dep(grad + p);
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (s_dot && row[k] >= 0) raw[i][k] = ld_dep(reinterpret_cast<const uint4*>(in + row[k] * in_pitch) + p);
     }
-    for (int p = threadIdx.x; p < pieces; p += blockDim.x) {
-      const uint4 raw_g = ld_dep(reinterpret_cast<const uint4*>(grad + t * grad_pitch) + p);
-      uint4 raw[TOP_K];
 #pragma unroll
-      for (int k = 0; k < TOP_K; ++k)
-        if (grad_w && row[k] >= 0) raw[k] = ld_dep(reinterpret_cast<const uint4*>(in + row[k] * in_pitch) + p);
-      float2 g[N];
-      unpack_piece<X>(raw_g, g);
+    for (int i = 0; i < U; ++i) {
+      const int p = p0 + i * blockDim.x;
+      if (p >= pieces) break;
+      float2 g[P];
+      unpack_piece<X>(raw_g[i], g);
 #pragma unroll
-      for (int k = 0; k < TOP_K; ++k) {
+      for (int k = 0; k < N; ++k) {
         if (row[k] < 0) continue;
-        if (grad_w) {
-          float2 f[N];
-          unpack_piece<X>(raw[k], f);
+        if (s_dot) {
+          float2 f[P];
+          unpack_piece<X>(raw[i][k], f);
 #pragma unroll
-          for (int j = 0; j < N; ++j) dot2[k] = fma2(g[j], f[j], dot2[k]);
+          for (int j = 0; j < P; ++j) dot2[k] = fma2(g[j], f[j], dot2[k]);
         }
         if (grad_in) {
-          float2 d[N];
+          float2 d[P];
 #pragma unroll
-          for (int j = 0; j < N; ++j) d[j] = mul2(both(w[k]), g[j]);
+          for (int j = 0; j < P; ++j) d[j] = mul2(both(w[k]), g[j]);
           reinterpret_cast<uint4*>(grad_in)[static_cast<long long>(row[k]) * pieces + p] = pack_piece<X>(d);
         }
       }
     }
+  }
+  if (!s_dot) return;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    float dot = dot2[k].x + dot2[k].y;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+    if ((threadIdx.x & 31) == 0) s_dot[k][threadIdx.x >> 5] = dot;
+  }
+}
+// One CTA per token (the dot products are sums over the whole row); either output may be absent.  THREADS: 256, three CTAs per
+// SM (110 registers and two: 320 us instead of 303 at 8192 tokens x 8 rows of 7168 bf16), or 512 for fewer tokens than SMs (64
+// tokens 5.1 us instead of 6.2).
+template <typename X, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
+k_token_combine_backward(const uint8_t* grad, long long grad_pitch, const uint8_t* in, long long in_pitch,
+                         const float* weights, int T, int K, int rows, int pieces, const int* row_pairs,
+                         const int* scatter_map, uint8_t* grad_in, float* grad_w) {
+  __shared__ float s_dot[TOP_K][16];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int t = blockIdx.x;
+  if (t < T) {
+    const TokenPairs pairs = token_pairs(scatter_map, weights, t, K, rows);
+    const uint4* grad_row = reinterpret_cast<const uint4*>(grad + t * grad_pitch);
+    if (pairs.mask && __popc(pairs.mask) <= 2)
+      combine_rows_backward<X, 2, 2>(grad_row, in, in_pitch, pairs, pieces, grad_in, grad_w ? s_dot : nullptr);
+    else if (pairs.mask)
+      combine_rows_backward<X, TOP_K, 1>(grad_row, in, in_pitch, pairs, pieces, grad_in, grad_w ? s_dot : nullptr);
     if (grad_w) {
-      float dot[TOP_K];
-#pragma unroll
-      for (int k = 0; k < TOP_K; ++k) dot[k] = dot2[k].x + dot2[k].y;
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1)
-#pragma unroll
-        for (int k = 0; k < TOP_K; ++k) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], d);
-      if ((threadIdx.x & 31) == 0)
-#pragma unroll
-        for (int k = 0; k < TOP_K; ++k) s_dot[k][threadIdx.x >> 5] = dot[k];
       __syncthreads();
       if (threadIdx.x < K) {
+        const uint32_t below = pairs.mask & ((1u << threadIdx.x) - 1u);
         float sum = 0.f;
-        for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) sum += s_dot[threadIdx.x][i];
+        if (pairs.mask >> threadIdx.x & 1u)
+          for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) sum += s_dot[__popc(below)][i];
         grad_w[static_cast<long long>(t) * K + threadIdx.x] = sum;
       }
     }
   }
-  if (grad_in) zero_unused_rows(row_pairs, rows, grad_in, pieces);
+  if (grad_in) zero_unused_rows(row_pairs, rows, grad_in, pieces, 0, pieces);
 }
 
 // w[t,k] = scale * s_k / (sum_j s_j + 1e-20) over the token's K selected experts, s = sigmoid(logit): the operations, and their
@@ -387,19 +455,29 @@ int launch_token_sort(const int* topk_idx, int T, int K, int E_local, int offset
   return B200MOE_OK;
 }
 
-// One CTA per token, more where the capacity has many rows per token.
+// One CTA per token, more where the capacity has many rows per token: at most nine rows per CTA to look through.
 static unsigned token_ctas(int T, int rows) {
   const int by_rows = (rows + TOP_K - 1) / TOP_K;
   return static_cast<unsigned>(T > by_rows ? T : by_rows);
 }
-static unsigned token_threads(int pieces) {
+static unsigned token_threads(int pieces, int most) {
   const int threads = (pieces + 31) / 32 * 32;
-  return static_cast<unsigned>(threads < 256 ? threads : 256);
+  return static_cast<unsigned>(threads < most ? threads : most);
+}
+// Parts of a row, a CTA each, while the batch alone does not fill the GPU: a call of few tokens is as long as a thread's chain of
+// loads and stores.  us with one CTA per token / with parts, at 7168 bf16 columns: gather of 1 token 3.9 / 2.3, of 333 tokens 14.8 /
+// 8.1; combine 3.1 / 1.6 and 6.1 / 5.0.  (Twice as many parts: 333 tokens 7.6 and 5.8.)
+constexpr unsigned TOKEN_FILL_CTAS = 592;   // four per SM
+static unsigned token_parts(unsigned ctas, int pieces, unsigned threads) {
+  const unsigned most = (pieces + threads - 1) / threads;
+  const unsigned want = (TOKEN_FILL_CTAS + ctas - 1) / ctas;
+  return want < most ? want : most;
 }
 
 int launch_token_gather(const void* x, long long x_pitch, int T, int K, int rows, int pieces, const int* row_pairs,
                         const int* scatter_map, void* out, cudaStream_t st) {
-  B200MOE_CUDA_TRY(launch_pdl(k_token_gather, dim3(token_ctas(T, rows)), dim3(token_threads(pieces)), 0, st,
+  const unsigned ctas = token_ctas(T, rows), threads = token_threads(pieces, 256);
+  B200MOE_CUDA_TRY(launch_pdl(k_token_gather, dim3(ctas, token_parts(ctas, pieces, threads)), dim3(threads), 0, st,
                               static_cast<const uint8_t*>(x), x_pitch, T, K, rows, pieces, row_pairs, scatter_map,
                               static_cast<uint8_t*>(out)));
   return B200MOE_OK;
@@ -415,7 +493,8 @@ static int with_row_type(int type, F&& f) {
 int launch_token_combine(const void* in, long long in_pitch, int type, const float* weights, int T, int K, int rows,
                          int pieces, const int* scatter_map, void* out, cudaStream_t st) {
   return with_row_type(type, [&](auto xt) -> int {
-    B200MOE_CUDA_TRY(launch_pdl(k_token_combine<decltype(xt)>, dim3(T), dim3(token_threads(pieces)), 0, st,
+    const unsigned threads = token_threads(pieces, 256);
+    B200MOE_CUDA_TRY(launch_pdl(k_token_combine<decltype(xt)>, dim3(T, token_parts(T, pieces, threads)), dim3(threads), 0, st,
                                 static_cast<const uint8_t*>(in), in_pitch, weights, K, rows, pieces, scatter_map,
                                 static_cast<uint8_t*>(out)));
     return B200MOE_OK;
@@ -426,10 +505,13 @@ int launch_token_combine_backward(const void* grad, long long grad_pitch, const 
                                   const float* weights, int T, int K, int rows, int pieces, const int* row_pairs,
                                   const int* scatter_map, void* grad_in, float* grad_w, cudaStream_t st) {
   return with_row_type(type, [&](auto xt) -> int {
-    B200MOE_CUDA_TRY(launch_pdl(k_token_combine_backward<decltype(xt)>, dim3(grad_in ? token_ctas(T, rows) : T),
-                                dim3(token_threads(pieces)), 0, st, static_cast<const uint8_t*>(grad), grad_pitch,
-                                static_cast<const uint8_t*>(in), in_pitch, weights, T, K, rows, pieces, row_pairs,
-                                scatter_map, static_cast<uint8_t*>(grad_in), grad_w));
+    using X = decltype(xt);
+    const bool few = T <= 148;
+    auto kern = few ? k_token_combine_backward<X, 512> : k_token_combine_backward<X, 256>;
+    B200MOE_CUDA_TRY(launch_pdl(kern, dim3(grad_in ? token_ctas(T, rows) : T), dim3(token_threads(pieces, few ? 512 : 256)),
+                                0, st, static_cast<const uint8_t*>(grad), grad_pitch, static_cast<const uint8_t*>(in),
+                                in_pitch, weights, T, K, rows, pieces, row_pairs, scatter_map,
+                                static_cast<uint8_t*>(grad_in), grad_w));
     return B200MOE_OK;
   });
 }

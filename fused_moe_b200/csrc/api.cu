@@ -284,8 +284,8 @@ int b200moe_token_sort(const int32_t* topk_idx, int32_t T, int32_t K, int32_t E_
   if (static_cast<long long>(T) * K + static_cast<long long>(E_local) * (align - 1) > B200MOE_TOKEN_MAX_ROWS)
     return B200MOE_EINVAL;
   if (!counts || !offsets || (rows > 0 && !row_pairs) || (T > 0 && (!topk_idx || !scatter_map))) return B200MOE_EINVAL;
-  if (scratch_bytes < token_sort_scratch_bytes(T, K, E_local)) return B200MOE_EWORKSPACE;
-  if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 3u)) return B200MOE_EWORKSPACE;
+  const size_t need = token_sort_scratch_bytes(T, K, E_local);
+  if (scratch_bytes < need || (need && !scratch) || (reinterpret_cast<uintptr_t>(scratch) & 3u)) return B200MOE_EWORKSPACE;
   int sms, rc;
   if ((rc = device_info(&sms))) return rc;
   return launch_token_sort(topk_idx, T, K, E_local, offset, align, rows, static_cast<int*>(scratch), counts, offsets,

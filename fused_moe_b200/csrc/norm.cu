@@ -248,11 +248,10 @@ k_add_rms_norm_backward(const uint8_t* grad_y, long long grad_y_pitch, const uin
   if (!partial) return;
   if (groups > 1) {   // the rows' space is free behind the barrier: it holds the sums of groups 1, 2, ... (checked by the host)
     __syncthreads();
-    uint8_t* sums = reinterpret_cast<uint8_t*>(s_rows);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int v = tid + i * row_threads;
-      if (group > 0 && v < n_vec) store_vec8<float>(sums, (group - 1) * n_vec + v, pack_vec8<float>(acc[i]));
+      if (group > 0 && v < n_vec) store_shared_vec8<float>(s_rows, (group - 1) * n_vec + v, pack_vec8<float>(acc[i]));
     }
     __syncthreads();
     if (group > 0) return;
@@ -311,7 +310,7 @@ k_norm_weight_grad(const float* partial, int rows, int columns, int type, void* 
   }
 }
 
-constexpr size_t MAX_DYNAMIC_SMEM = 227 * 1024 - 1024;   // of a CTA, less the static arrays
+constexpr int MAX_DYNAMIC_SMEM = 227 * 1024 - 1024;   // of a CTA, less the static arrays
 
 // Vectors of eight columns per thread.  Forward: few tokens want many threads each (a CTA's latency is the call's), many tokens
 // few and fat ones (the row's sum costs per warp).  us at 7168 columns, two / four vectors: 1 token 2.3 / 2.8, 333 tokens
@@ -390,13 +389,27 @@ int launch_add_rms_norm_backward(const void* grad_y, long long grad_y_pitch, int
     const size_t stage = static_cast<size_t>(columns) * (sizeof(X) + sizeof(R) * (grad_stream ? 2 : 1));
     // tokens that a CTA works on at once: about BACKWARD_THREADS threads' worth
     const int groups = s.threads >= BACKWARD_THREADS ? 1 : BACKWARD_THREADS / s.threads;
-    auto launch = [&](auto kern, int stages) -> int {
+    auto launch = [&](auto stages, auto is_exact) -> int {
+      auto kern = k_add_rms_norm_backward<X, R, W, VPT, decltype(stages)::value, decltype(is_exact)::value>;
       const size_t smem = stage * stages * groups;
       static_assert(sizeof(X) + sizeof(R) >= 4, "two stages of a row hold its columns in float32: the groups' sums fit");
-      B200MOE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-      int per_sm = 0;
-      B200MOE_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, s.threads * groups, smem));
-      int most = num_sms * (per_sm > 0 ? per_sm : 1);
+      // this kernel's last answer to this thread is kept (a lambda of its own, and so a variable, for each pair of tags): the two
+      // calls take microseconds
+      static thread_local struct {
+        int device = -1, threads = 0, per_sm = 0;
+        size_t smem = 0;
+      } known;
+      int device = 0;
+      B200MOE_CUDA_TRY(cudaGetDevice(&device));
+      if (known.device != device || known.threads != s.threads * groups || known.smem != smem) {
+        known.device = -1;
+        B200MOE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_DYNAMIC_SMEM));
+        B200MOE_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&known.per_sm, kern, s.threads * groups, smem));
+        known.device = device;
+        known.threads = s.threads * groups;
+        known.smem = smem;
+      }
+      int most = num_sms * (known.per_sm > 0 ? known.per_sm : 1);
       if (most > B200MOE_NORM_PARTIAL_ROWS) most = B200MOE_NORM_PARTIAL_ROWS;
       const int batches = (T + groups - 1) / groups;
       const int rounds = (batches + most - 1) / most;   // of the busiest CTA; no more CTAs than that takes
@@ -410,10 +423,10 @@ int launch_add_rms_norm_backward(const void* grad_y, long long grad_y_pitch, int
       return B200MOE_OK;
     };
     const bool exact = s.n_vec == VPT * s.threads;
-    if (2 * stage * groups <= MAX_DYNAMIC_SMEM)
-      return exact ? launch(k_add_rms_norm_backward<X, R, W, VPT, 2, true>, 2)
-                   : launch(k_add_rms_norm_backward<X, R, W, VPT, 2, false>, 2);
-    return launch(k_add_rms_norm_backward<X, R, W, VPT, 1, false>, 1);
+    if (2 * stage * groups <= static_cast<size_t>(MAX_DYNAMIC_SMEM))
+      return exact ? launch(std::integral_constant<int, 2>(), std::true_type())
+                   : launch(std::integral_constant<int, 2>(), std::false_type());
+    return launch(std::integral_constant<int, 1>(), std::false_type());
   });
   if (rc || !grad_weight) return rc;
   B200MOE_CUDA_TRY(launch_pdl(k_norm_weight_grad, dim3((columns + 31) / 32), dim3(WEIGHT_GRAD_WARPS * 32), 0, st,

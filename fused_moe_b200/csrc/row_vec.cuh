@@ -115,7 +115,7 @@ __device__ __forceinline__ void store_vec8(uint8_t* row, int v, const Vec8<T>& r
 #pragma unroll
   for (int i = 0; i < Vec8<T>::PIECES; ++i) reinterpret_cast<uint4*>(row)[v * Vec8<T>::PIECES + i] = r.p[i];
 }
-// The same through shared memory: an asynchronous copy into it, and a read.
+// The same through shared memory: an asynchronous copy into it, a store, a read.
 template <typename T>
 __device__ __forceinline__ void copy_vec8(uint32_t slot, const uint8_t* row, int v) {
 #pragma unroll
@@ -123,6 +123,11 @@ __device__ __forceinline__ void copy_vec8(uint32_t slot, const uint8_t* row, int
     const int at = (v * Vec8<T>::PIECES + i) * 16;
     cp_async16(slot + at, row + at);
   }
+}
+template <typename T>
+__device__ __forceinline__ void store_shared_vec8(uint4* slot, int v, const Vec8<T>& r) {
+#pragma unroll
+  for (int i = 0; i < Vec8<T>::PIECES; ++i) slot[v * Vec8<T>::PIECES + i] = r.p[i];
 }
 template <typename T>
 __device__ __forceinline__ Vec8<T> shared_vec8(const uint4* slot, int v) {

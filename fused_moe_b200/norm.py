@@ -27,10 +27,9 @@ def _check(x, residual, weight, eps, multiple: int, names=("x", "residual")) -> 
     if T > MAX_TOKENS:
         raise ValueError(f"{names[0]} must have at most {MAX_TOKENS} rows")
     if residual is not None:
-        if torch.is_tensor(residual) and residual.dtype is not x.dtype and residual.dtype is not torch.float32:
-            raise TypeError(f"{names[1]} must have the type of {names[0]} or float32, got {residual.dtype}")
-        check_tensor(residual, names[1], residual.dtype if torch.is_tensor(residual) else x.dtype, (T, columns))
-    if not torch.is_tensor(weight) or (weight.dtype is not x.dtype and weight.dtype is not torch.float32):
+        wide = isinstance(residual, torch.Tensor) and residual.dtype is torch.float32
+        check_tensor(residual, names[1], torch.float32 if wide else x.dtype, (T, columns))
+    if not isinstance(weight, torch.Tensor) or (weight.dtype is not x.dtype and weight.dtype is not torch.float32):
         raise TypeError(f"weight must be a tensor of the type of {names[0]} or float32")
     check_tensor(weight, "weight", weight.dtype, (columns,))
     if not eps >= 0.0:
@@ -100,8 +99,8 @@ class _AddRmsNorm(torch.autograd.Function):
     @staticmethod
     @differentiable_once
     def backward(ctx, grad_y, grad_stream=None):
-        refuse_capture("add_rms_norm_backward")
         stream, weight = ctx.saved_tensors
+        refuse_capture("add_rms_norm_backward", stream.device)
         need_x, need_residual, need_weight = ctx.needs_input_grad[:3]
         if grad_y is None:   # only the residual stream was used: it passes its gradient on
             if grad_stream is None:
@@ -138,7 +137,7 @@ def add_rms_norm_backward(grad_y: torch.Tensor, grad_stream: Optional[torch.Tens
     None, ``grad_stream``; ``stream`` is the r that the forward call returned.  grad_x has the type of ``grad_y``,
     grad_residual that of ``stream`` (the same tensor where the types are equal), grad_weight that of ``weight``.  It
     runs no autograd and allocates nothing but its results and scratch, so it can be captured into a CUDA graph."""
-    if not torch.is_tensor(stream):
+    if not isinstance(stream, torch.Tensor):
         raise TypeError("stream must be a torch.Tensor")
     shape = _check(grad_y, stream, weight, eps, 8, ("grad_y", "stream"))
     if grad_stream is not None:

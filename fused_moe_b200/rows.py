@@ -7,7 +7,6 @@ import functools
 from typing import Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .kernel import _require_cuda
@@ -18,21 +17,22 @@ MAX_TOKENS = 1 << 24
 
 def check_rows(t, name: str) -> Tuple[int, int]:
     """(rows, columns) of a 2-d tensor of bf16, f16 or f32."""
-    if not torch.is_tensor(t):
+    if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype not in DTYPES:
         raise TypeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
-    if t.dim() != 2:
-        raise ValueError(f"{name} must have two dimensions, got {tuple(t.shape)}")
-    return int(t.shape[0]), int(t.shape[1])
+    shape = t.shape
+    if len(shape) != 2:
+        raise ValueError(f"{name} must have two dimensions, got {tuple(shape)}")
+    return shape[0], shape[1]
 
 
 def check_tensor(t, name: str, dtype: torch.dtype, shape: Tuple[int, ...]) -> None:
-    if not torch.is_tensor(t):
+    if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
 
 
@@ -81,14 +81,30 @@ def stream_of(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def differentiable_once(backward):
-    """``once_differentiable`` for the pass that asks for a second derivative only: its wrapper costs microseconds, and without
-    one (gradients are then not being recorded) it does nothing."""
-    guarded = once_differentiable(backward)
+class _FirstDerivative(torch.autograd.Function):
+    """Passes gradients on; differentiating them raises."""
 
+    @staticmethod
+    def forward(ctx, anchor, *grads):
+        return tuple(None if g is None else g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("the operators around the layer are differentiable once: a second derivative is not available")
+
+
+def differentiable_once(backward):
+    """For the backward pass of an autograd function: where gradients are recorded (``create_graph=True``) its results raise when
+    they are differentiated in turn.  (torch's own ``once_differentiable`` does so only where the incoming gradients
+    require one; the results of a constant gradient would count as constants of the inputs.)"""
     @functools.wraps(backward)
     def call(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            results = backward(ctx, *grads)
+        results = results if isinstance(results, tuple) else (results,)
+        return _FirstDerivative.apply(torch.empty(0, requires_grad=True), *results)
     return call
 
 
@@ -99,12 +115,14 @@ def records_graph(instead: str, *tensors) -> bool:
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
-                refuse_capture(instead)
+                refuse_capture(instead, t.device)
                 return True
     return False
 
 
-def refuse_capture(instead: str) -> None:
-    if torch.cuda.is_current_stream_capturing():
+def refuse_capture(instead: str, device: torch.device) -> None:
+    with on_device(device):
+        capturing = torch.cuda.is_current_stream_capturing()
+    if capturing:
         raise RuntimeError("autograd is not available during stream capture: capture the call under torch.no_grad() and "
                            f"its gradient as {instead}(...)")

@@ -13,8 +13,7 @@ sorts, :1758-1821 reduces); the reference has no gradient.
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -24,8 +23,7 @@ from .rows import DTYPES, MAX_TOKENS, check_device, check_rows, check_tensor, de
     records_graph, refuse_capture, row_pointer, stream_of
 
 
-@dataclass(frozen=True)
-class TokenSort:
+class TokenSort(NamedTuple):
     """Where each (token, k) pair of a batch goes.  Device tensors of int32; nothing here was read by the host.
 
     counts [E]          pairs of each local expert (those without a row among them, see ``rows``)
@@ -44,13 +42,14 @@ class TokenSort:
 
 
 def _selection(topk_idx) -> tuple:
-    if not torch.is_tensor(topk_idx):
+    if not isinstance(topk_idx, torch.Tensor):
         raise TypeError("topk_idx must be a torch.Tensor")
     if topk_idx.dtype is not torch.int32:
         raise TypeError(f"topk_idx must be torch.int32, got {topk_idx.dtype}")
-    if topk_idx.dim() != 2 or not 1 <= topk_idx.shape[1] <= TOP_K or topk_idx.shape[0] > MAX_TOKENS:
-        raise ValueError(f"topk_idx must be [T, K] with K in 1..{TOP_K} and T <= {MAX_TOKENS}, got {tuple(topk_idx.shape)}")
-    return int(topk_idx.shape[0]), int(topk_idx.shape[1])
+    shape = topk_idx.shape
+    if len(shape) != 2 or not 1 <= shape[1] <= TOP_K or shape[0] > MAX_TOKENS:
+        raise ValueError(f"topk_idx must be [T, K] with K in 1..{TOP_K} and T <= {MAX_TOKENS}, got {tuple(shape)}")
+    return shape[0], shape[1]
 
 
 def sort_tokens(topk_idx: torch.Tensor, E_local: int, local_expert_offset=0, align: int = 1,
@@ -83,9 +82,10 @@ def sort_tokens(topk_idx: torch.Tensor, E_local: int, local_expert_offset=0, ali
     _lib.check(lib.b200moe_token_sort_scratch_bytes(T, K, E_local, C.byref(need)), "b200moe_token_sort_scratch_bytes")
     ints = topk_idx.new_empty
     plan = TokenSort(ints(E_local), ints(E_local + 1), ints(rows), ints((T, K)), rows, align)
-    scratch = ints(need.value // 4)
+    scratch = ints(need.value // 4) if need.value else None   # a small batch needs none
     with on_device(device):
-        _lib.check(lib.b200moe_token_sort(idx.data_ptr(), T, K, E_local, offset, align, rows, scratch.data_ptr(), need.value,
+        _lib.check(lib.b200moe_token_sort(idx.data_ptr(), T, K, E_local, offset, align, rows,
+                                          None if scratch is None else scratch.data_ptr(), need.value,
                                           plan.counts.data_ptr(), plan.offsets.data_ptr(), plan.row_pairs.data_ptr(),
                                           plan.scatter_map.data_ptr(), stream_of(device)),
                    "b200moe_token_sort")
@@ -155,7 +155,7 @@ class _GatherTokens(torch.autograd.Function):
     @staticmethod
     @differentiable_once
     def backward(ctx, grad):
-        refuse_capture("gather_tokens_backward")
+        refuse_capture("gather_tokens_backward", grad.device)
         return _combine(grad, None, *ctx.saved_tensors), None
 
 
@@ -169,7 +169,7 @@ class _CombineTokens(torch.autograd.Function):
     @staticmethod
     @differentiable_once
     def backward(ctx, grad):
-        refuse_capture("combine_tokens_backward")
+        refuse_capture("combine_tokens_backward", grad.device)
         rows, weights, row_pairs, scatter_map = ctx.saved_tensors
         return (*_combine_backward(grad, rows, weights, row_pairs, scatter_map, *ctx.needs_input_grad[:2]), None)
 
@@ -195,7 +195,7 @@ def gather_tokens_backward(grad: torch.Tensor, plan: TokenSort) -> torch.Tensor:
 
 
 def _check_weights(weights, plan: TokenSort, first: torch.Tensor) -> None:
-    check_tensor(weights, "topk_weights", torch.float32, tuple(plan.scatter_map.shape))
+    check_tensor(weights, "topk_weights", torch.float32, plan.scatter_map.shape)
     check_device(first, weights)
 
 
@@ -265,7 +265,7 @@ class _RouteWeights(torch.autograd.Function):
     @staticmethod
     @differentiable_once
     def backward(ctx, grad):
-        refuse_capture("route_weights_backward")
+        refuse_capture("route_weights_backward", grad.device)
         return _route_weights_backward(*ctx.saved_tensors, grad, ctx.scale), None, None
 
 

@@ -238,7 +238,8 @@ int b200moe_add_rms_norm_backward(const void* grad_y, int64_t grad_y_pitch, int3
  *   offsets [E_local + 1]  first row of each segment and the end of the last, at most `rows`
  *   row_pairs [rows]       pair of each row, -1 for a row without one
  *   scatter_map [T, K]     row of each pair, -1 for a pair without one
- * scratch: b200moe_token_sort_scratch_bytes(T, K, E_local) bytes, 4-byte aligned, not shared with a call in flight. */
+ * scratch: b200moe_token_sort_scratch_bytes(T, K, E_local) bytes (0 for a small batch), 4-byte aligned, not shared with a
+ * call in flight. */
 #define B200MOE_TOKEN_SORT_MAX_CTAS 256
 #define B200MOE_TOKEN_MAX_ROWS (1 << 30)
 int b200moe_token_sort_scratch_bytes(int32_t T, int32_t K, int32_t E_local, size_t* bytes /* host */);

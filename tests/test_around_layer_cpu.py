@@ -216,6 +216,9 @@ def test_token_abi_refuses(lib):
                    dict(rows=(1 << 30) + 1), dict(align=1 << 26), dict(counts=None), dict(offsets=None),
                    dict(row_pairs=None), dict(map=None)):
         assert lib.b200moe_token_sort(*with_args(base, **change)) == _lib.EINVAL, change
+    assert lib.b200moe_token_sort_scratch_bytes(8, 8, 32, C.byref(n)) == 0 and n.value == 0
+    base.update(T=4096)
+    assert lib.b200moe_token_sort_scratch_bytes(4096, 8, 32, C.byref(n)) == 0 and n.value > 4
     for change in (dict(scratch=None), dict(scratch=A + 2), dict(bytes=4)):
         assert lib.b200moe_token_sort(*with_args(base, **change)) == _lib.EWORKSPACE, change
     base = dict(x=A, pitch=0, type=0, T=8, K=8, columns=64, rows=64, row_pairs=A, map=A, out=A, stream=None)

@@ -347,7 +347,7 @@ def test_refuses_an_autograd_pass_under_capture(norm):
         held += 1
         with pytest.raises(RuntimeError, match="stream capture"):
             from fused_moe_b200 import rows
-            rows.refuse_capture("add_rms_norm_backward")   # what the backward pass calls first
+            rows.refuse_capture("add_rms_norm_backward", x.device)   # what the backward pass calls first
     graph.replay()
     torch.cuda.synchronize()
     assert held.eq(1).all()
@@ -375,3 +375,14 @@ def test_feeds_the_layer(norm, oracle, T):
     want = oracle.kernel(*[args[k].cpu() if torch.is_tensor(args[k]) else args[k] for k in keys])
     assert want["pairs"] > 0 and r.isfinite().all()
     assert_close(out.cpu(), want["out_f32"])
+
+
+def test_second_derivatives_are_refused(norm):
+    """Also where the first gradient came from a constant: it must not pass for a constant of the inputs."""
+    x, res, w, rnd = make(3, 128, F32, F32, seed=17)
+    x.requires_grad_()
+    y, _ = norm.add_rms_norm(x, res, w)
+    g = torch.autograd.grad(y.sum(), x, create_graph=True)[0]
+    assert torch.equal(g, norm.add_rms_norm_backward(torch.ones_like(y), None, (x + res).detach(), w)[0])
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (g.sum() + x.square().sum()).backward()

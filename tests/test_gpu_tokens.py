@@ -233,6 +233,17 @@ def test_partial_gradients(tok):
     assert torch.equal(one, tok.combine_tokens_backward(torch.ones_like(gy), h, w, plan)[0])
 
 
+def test_second_derivatives_are_refused(tok):
+    idx = select(6, 8, 15)
+    plan = tok.sort_tokens(idx, 256)
+    x, h, w, logits = (torch.randn(s, device="cuda").requires_grad_() for s in ((6, 64), (48, 64), (6, 8), (6, 256)))
+    for out, leaves in ((tok.gather_tokens(x, plan), (x,)), (tok.combine_tokens(h, w, plan), (h, w)),
+                        (tok.route_weights(logits, idx, 2.5), (logits,))):
+        grads = torch.autograd.grad(out.square().sum(), leaves, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            sum((g.sum() + leaf.square().sum()) for g, leaf in zip(grads, leaves)).backward()
+
+
 def test_strided_and_unaligned_rows(tok):
     idx = select(30, 8, 10, "padded")
     plan = tok.sort_tokens(idx, 256, align=16)
@@ -249,18 +260,17 @@ def test_strided_and_unaligned_rows(tok):
 
 def test_rows_of_another_batch_do_no_harm(tok):
     """A map whose entries lie outside the buffers: such a pair counts as one without a row."""
-    from dataclasses import replace
     plan = tok.sort_tokens(select(10, 8, 11), 256)
     bad = plan.scatter_map.clone()
     bad[0, 0], bad[1, 1], bad[2, 2] = 80, -7, 2 ** 31 - 1
     x, w = torch.randn(10, 64, device="cuda"), torch.randn(10, 8, device="cuda")
     h = torch.randn(80, 64, device="cuda")
     keep = (bad >= 0) & (bad < 80)
-    got = tok.combine_tokens(h, w, replace(plan, scatter_map=bad))
+    got = tok.combine_tokens(h, w, plan._replace(scatter_map=bad))
     want = (torch.where(keep[:, :, None], h[torch.where(keep, bad, 0).long()], 0.0).double() * w.double()[:, :, None])
     assert_within(got, want.sum(dim=1), 9 * EPS24 * want.abs().sum(dim=1), "combined")
-    assert tok.gather_tokens(x, replace(plan, scatter_map=bad)).shape == (80, 64)
-    assert tok.combine_tokens_backward(x, h, w, replace(plan, scatter_map=bad))[1][~keep].eq(0).all()
+    assert tok.gather_tokens(x, plan._replace(scatter_map=bad)).shape == (80, 64)
+    assert tok.combine_tokens_backward(x, h, w, plan._replace(scatter_map=bad))[1][~keep].eq(0).all()
     torch.cuda.synchronize()
 
 

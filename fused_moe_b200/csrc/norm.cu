@@ -9,7 +9,13 @@
 //   dr = rstd * (g - r * rstd^2 * mean(g * r)) + dr_out       dweight = sum over tokens of dy * r * rstd
 // rstd is recomputed: sum(r^2) and sum(g * r) are taken in the same pass over the row.
 //
-// Sums and statistics are float32.  All kernels are bound by the bytes of the rows.
+// Sums and statistics are float32.
+//
+// Bound by the bytes of the rows once the instructions are out of the way: a first form with one float32 operation per
+// instruction, predicated vectors and the weight's type looked up at run time issued 31 (forward, e4m3) and 43 (backward) warp
+// instructions per element and lane and ran at 5.5 and 3.7 TB/s; paired operations, types as template arguments and rows of
+// whole vectors brought 16384 x 7168 bf16 to 124 us with e4m3 out (826 MB: 6.6 TB/s; 132 - 139 in a long run, where the
+// clocks settle lower), 137 us with bf16 out (940 MB) and 146 us backward (940 MB and the partial sums).
 #include <type_traits>
 
 #include "row_vec.cuh"
@@ -23,8 +29,8 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;
 }
-// Two sums over the warp for the price of little more than one: after the first exchange lanes 0..15 hold half sums of `a` and lanes
-// 16..31 of `b`.  Returns the half-warp's own sum.
+// Two sums over the warp for the price of little more than one: after the first exchange lanes 0..15 hold half sums of `a`
+// and lanes 16..31 of `b`.  Returns the half-warp's own sum.
 __device__ __forceinline__ float warp_sum_halves(float a, float b) {
   const bool upper = threadIdx.x & 16;
   float v = (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
@@ -55,8 +61,11 @@ __device__ __forceinline__ float max_abs_nan(float m, float a) {
   return d;
 }
 
-// A row is VPT vectors of eight columns per thread, as many vectors apart as the row has threads, so that a half-warp holds a whole 128-column
-// block.  WARP_ROW: a warp per token, several tokens per CTA, and no barrier; else one CTA per token.
+// One pass: a row is read once, kept in registers across the sum, and written.  What hides the latency of a row's load behind
+// other rows' stores is several CTAs per SM, not a pipeline inside one.
+//
+// A row is VPT vectors of eight columns per thread, as many vectors apart as the row has threads, so that a half-warp holds a
+// whole 128-column block.  WARP_ROW: a warp per token, several tokens per CTA, and no barrier; else one CTA per token.
 template <typename X, typename R, typename W, int VPT, bool WARP_ROW>
 __global__ void __launch_bounds__(MAX_WARPS * 32)
 k_add_rms_norm(const uint8_t* x, long long x_pitch, const uint8_t* residual, long long residual_pitch,
@@ -118,8 +127,8 @@ k_add_rms_norm(const uint8_t* x, long long x_pitch, const uint8_t* residual, lon
       float m = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) m = max_abs_nan(max_abs_nan(m, r[i][j].x), r[i][j].y);
-      // patterns of non-negative floats order like the floats, and a NaN (as max.NaN gives it) is above them all: it then stands in
-      // the scale too
+      // patterns of non-negative floats order like the floats, and a NaN (as max.NaN gives it) is above them all: it then
+      // stands in the scale too
       const float amax =
           __uint_as_float(__reduce_max_sync((threadIdx.x & 16) ? 0xffff0000u : 0x0000ffffu, __float_as_uint(m)));
       float s = __fmul_rn(amax, 1.0f / 448.0f);
@@ -134,14 +143,18 @@ k_add_rms_norm(const uint8_t* x, long long x_pitch, const uint8_t* residual, lon
   }
 }
 
-// A CTA works on `groups` tokens at a time, `row_threads` threads each (narrow rows: several; wide rows: one), grid-stride over the
-// tokens.  A thread keeps its columns, so dweight accumulates in registers over the CTA's tokens; the groups' sums are added in
-// order at the end and leave as one float32 row of `partial` per CTA.  Fixed order of every sum: two runs give the same bits.
+// A CTA works on `groups` tokens at a time, `row_threads` threads each (narrow rows: several; wide rows: one), grid-stride
+// over the tokens.  A thread keeps its columns, so dweight accumulates in registers over the CTA's tokens; the groups' sums
+// are added in order at the end and leave as one float32 row of `partial` per CTA.  Fixed order of every sum: two runs give
+// the same bits.
 //
 // The rows of a group's next STAGES - 1 tokens are under way in shared memory (16-byte asynchronous copies) while one is worked
 // on: a row's two passes (sums, then output) have a sum over its threads between them, in which nothing would be loaded
 // otherwise.  A thread copies exactly the pieces that it reads itself, so its own wait orders them and the pipeline needs no
-// barrier.
+// barrier.  Two stages; a third costs the second CTA per SM (16384 x 7168 bf16: 289 us against 209, when the rest was slower).
+//
+// EXACT: every thread has VPT vectors (7168 columns: 4 x 224 threads), so that no vector is predicated: with the weight kept in
+// registers, 8192 x 7168 bf16 94 -> 79 us.
 template <typename X, typename R, typename W, int VPT, int STAGES, bool EXACT>
 __global__ void __launch_bounds__(MAX_WARPS * 32)
 k_add_rms_norm_backward(const uint8_t* grad_y, long long grad_y_pitch, const uint8_t* grad_stream,
@@ -276,7 +289,8 @@ k_add_rms_norm_backward(const uint8_t* grad_y, long long grad_y_pitch, const uin
   }
 }
 
-// dweight[c] = sum of the rows of `partial`, rounded once: 32 columns per CTA, its warps take the rows in turn, sixteen in flight.
+// dweight[c] = sum of the rows of `partial`, rounded once: 32 columns per CTA, its warps take the rows in turn, sixteen in
+// flight.
 constexpr int WEIGHT_GRAD_WARPS = 16;
 __global__ void __launch_bounds__(WEIGHT_GRAD_WARPS * 32)
 k_norm_weight_grad(const float* partial, int rows, int columns, int type, void* grad_weight) {
@@ -393,8 +407,8 @@ int launch_add_rms_norm_backward(const void* grad_y, long long grad_y_pitch, int
       auto kern = k_add_rms_norm_backward<X, R, W, VPT, decltype(stages)::value, decltype(is_exact)::value>;
       const size_t smem = stage * stages * groups;
       static_assert(sizeof(X) + sizeof(R) >= 4, "two stages of a row hold its columns in float32: the groups' sums fit");
-      // this kernel's last answer to this thread is kept (a lambda of its own, and so a variable, for each pair of tags): the two
-      // calls take microseconds
+      // this kernel's last answer to this thread is kept (a lambda of its own, and so a variable, for each pair of tags): the
+      // two calls take microseconds
       static thread_local struct {
         int device = -1, threads = 0, per_sm = 0;
         size_t smem = 0;

@@ -1,5 +1,6 @@
-// Rows of bf16, f16 or f32 elements in 16-byte pieces: loads below the dependency wait, conversion to float32 and back (round to
-// nearest even), stores.  Used by the norm and token-permutation kernels, which take the element type as a template argument.
+// Rows of bf16, f16 or f32 elements in 16-byte pieces: loads below the dependency wait, conversion to float32 and back (round
+// to nearest even), stores.  Used by the norm and token-permutation kernels, which take the element type as a template
+// argument.
 //
 // Values are held and computed in pairs: sm_100 multiplies, adds and fuses two float32 per instruction, each rounded as by
 // itself.  The kernels here stream rows at the memory's rate, where issue slots are what runs out next.

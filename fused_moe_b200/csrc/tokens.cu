@@ -45,9 +45,9 @@ k_token_count(const int* topk_idx, long long n_pairs, long long per, int offset,
   if (threadIdx.x < E_local) hist[blockIdx.x * E_local + threadIdx.x] = s_count[threadIdx.x];
 }
 
-// The rows: every CTA derives the layout from the counts of all CTAs (`hist`, or for a small batch, hist == nullptr, by counting
-// the whole batch itself, which saves the launch of k_token_count), then ranks its pairs SORT_THREADS at a time.  Inside a
-// warp the rank is the number of lower lanes with the same expert, and the warps' counts are prefixed per expert.
+// The rows: every CTA derives the layout from the counts of all CTAs (`hist`, or for a small batch, hist == nullptr, by
+// counting the whole batch itself, which saves the launch of k_token_count), then ranks its pairs SORT_THREADS at a time.
+// Inside a warp the rank is the number of lower lanes with the same expert, and the warps' counts are prefixed per expert.
 __global__ void __launch_bounds__(SORT_THREADS)
 k_token_place(const int* topk_idx, long long n_pairs, long long per, int offset, int E_local, int align, int rows,
               const int* hist, int* counts, int* offsets, int* row_pairs, int* scatter_map) {
@@ -146,8 +146,9 @@ k_token_place(const int* topk_idx, long long n_pairs, long long per, int offset,
   }
 }
 
-// A token's pairs, one per lane of every warp: lane k < K holds the row (-1: none; an entry outside 0 .. rows - 1 is none, so that
-// a map of another batch cannot lead a store out of the buffer) and the weight of pair (t, k).  `mask`: the lanes with a row.
+// A token's pairs, one per lane of every warp: lane k < K holds the row (-1: none; an entry outside 0 .. rows - 1 is none, so
+// that a map of another batch cannot lead a store out of the buffer) and the weight of pair (t, k).  `mask`: the lanes with a
+// row.
 struct TokenPairs {
   int row;
   float weight;
@@ -387,42 +388,50 @@ k_route_weights(const float* logits, const int* topk_idx, int T, int K, float sc
 
 // With S = sum_j s_j + 1e-20 and g = the weights' gradient:
 //   grad_logit_k = s_k * (1 - s_k) * scale / S * (g_k - sum_j g_j s_j / S),  every other column 0.
-// 1 - sigmoid(x) is taken as sigmoid(-x), which loses nothing where s is near 1.  A warp per token; an expert named twice gets
-// both terms, in the order of k.
-__global__ void __launch_bounds__(256)
+// 1 - sigmoid(x) is taken as sigmoid(-x), which loses nothing where s is near 1.  A warp works on four tokens, eight lanes each,
+// and puts their rows together in shared memory; an expert named twice gets both terms, added in the order of k by the first
+// lane that names it.  (A warp per token with the columns in registers: 16384 tokens 7.7 us, now 6.5.)
+constexpr int ROUTE_GRAD_WARPS = 8, ROUTE_GRAD_TOKENS = 4;
+__global__ void __launch_bounds__(ROUTE_GRAD_WARPS * 32)
 k_route_weights_backward(const float* logits, const int* topk_idx, const float* grad, int T, int K, float scale,
                          float* grad_logits) {
+  __shared__ float4 s_rows[ROUTE_GRAD_WARPS][ROUTE_GRAD_TOKENS * E_GLOBAL / 4];
   pdl_launch_dependents();
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const long long t = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (t >= T) return;
-  const int id = lane < K ? ld_dep(topk_idx + t * K + lane) : -1;
-  const float g = lane < K ? ld_dep(grad + t * K + lane) : 0.f;
-  const float s = selected_sigmoid(logits, t, id, 1.f), c = selected_sigmoid(logits, t, id, -1.f);
-  float total = s, mix = static_cast<uint32_t>(id) < static_cast<uint32_t>(E_GLOBAL) ? g * s : 0.f;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = lane % TOP_K;
+  constexpr int PIECES = ROUTE_GRAD_TOKENS * E_GLOBAL / 4 / 32;   // of the four rows, per lane
+  float4* rows = s_rows[warp];
 #pragma unroll
-  for (int d = 4; d > 0; d >>= 1) {   // lanes 0..7
+  for (int i = 0; i < PIECES; ++i) rows[i * 32 + lane] = make_float4(0.f, 0.f, 0.f, 0.f);
+  pdl_wait();
+  const long long t0 = (static_cast<long long>(blockIdx.x) * ROUTE_GRAD_WARPS + warp) * ROUTE_GRAD_TOKENS;
+  const long long t = t0 + lane / TOP_K;
+  const bool live = t < T && k < K;
+  const int id = live ? ld_dep(topk_idx + t * K + k) : -1;
+  const bool valid = static_cast<uint32_t>(id) < static_cast<uint32_t>(E_GLOBAL);
+  const float g = live ? ld_dep(grad + t * K + k) : 0.f;
+  const float s = selected_sigmoid(logits, t, id, 1.f), c = selected_sigmoid(logits, t, id, -1.f);
+  float total = s, mix = valid ? g * s : 0.f;
+#pragma unroll
+  for (int d = TOP_K / 2; d > 0; d >>= 1) {
     total += __shfl_xor_sync(0xffffffffu, total, d);
     mix += __shfl_xor_sync(0xffffffffu, mix, d);
   }
   total += 1e-20f;
   const float grad_k = s * c * (scale / total) * (g - mix / total);
-  float out[8];
+  const uint32_t same = __match_any_sync(0xffffffffu, valid ? (lane / TOP_K) * E_GLOBAL + id : -1 - lane);
+  float sum = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) out[j] = 0.f;
-#pragma unroll
-  for (int k = 0; k < TOP_K; ++k) {
-    const int e = __shfl_sync(0xffffffffu, id, k);
-    const float d = __shfl_sync(0xffffffffu, grad_k, k);
-    if (static_cast<uint32_t>(e) >= static_cast<uint32_t>(E_GLOBAL)) continue;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)   // column 4 * lane + 128 * (j / 4) + j % 4
-      if (e == 4 * lane + 128 * (j >> 2) + (j & 3)) out[j] += d;
+  for (int j = 0; j < TOP_K; ++j) {
+    const float v = __shfl_sync(0xffffffffu, grad_k, j, TOP_K);
+    if (same >> ((lane & ~(TOP_K - 1)) + j) & 1u) sum += v;
   }
-  float4* dst = reinterpret_cast<float4*>(grad_logits + t * E_GLOBAL);
-  dst[lane] = make_float4(out[0], out[1], out[2], out[3]);
-  dst[32 + lane] = make_float4(out[4], out[5], out[6], out[7]);
+  __syncwarp();
+  if (valid && __ffs(same) - 1 == lane) reinterpret_cast<float*>(rows)[(lane / TOP_K) * E_GLOBAL + id] = sum;
+  __syncwarp();
+  float4* dst = reinterpret_cast<float4*>(grad_logits + t0 * E_GLOBAL);
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i)   // piece i * 32 + lane is of token i * 32 / 64
+    if (t0 + i * 32 / (E_GLOBAL / 4) < T) dst[i * 32 + lane] = rows[i * 32 + lane];
 }
 
 // Pairs per CTA and CTAs of the sort: whole rounds of SORT_THREADS pairs, at most SORT_MAX_CTAS CTAs.
@@ -463,9 +472,9 @@ static unsigned token_threads(int pieces, int most) {
   const int threads = (pieces + 31) / 32 * 32;
   return static_cast<unsigned>(threads < most ? threads : most);
 }
-// Parts of a row, a CTA each, while the batch alone does not fill the GPU: a call of few tokens is as long as a thread's chain of
-// loads and stores.  us with one CTA per token / with parts, at 7168 bf16 columns: gather of 1 token 3.9 / 2.3, of 333 tokens 14.8 /
-// 8.1; combine 3.1 / 1.6 and 6.1 / 5.0.  (Twice as many parts: 333 tokens 7.6 and 5.8.)
+// Parts of a row, a CTA each, while the batch alone does not fill the GPU: a call of few tokens is as long as a thread's
+// chain of loads and stores.  us with one CTA per token / with parts, at 7168 bf16 columns: gather of 1 token 3.9 / 2.3, of
+// 333 tokens 14.8 / 8.1; combine 3.1 / 1.6 and 6.1 / 5.0.  (Twice as many parts: 333 tokens 7.6 and 5.8.)
 constexpr unsigned TOKEN_FILL_CTAS = 592;   // four per SM
 static unsigned token_parts(unsigned ctas, int pieces, unsigned threads) {
   const unsigned most = (pieces + threads - 1) / threads;
@@ -524,7 +533,9 @@ int launch_route_weights(const float* logits, const int* topk_idx, int T, int K,
 
 int launch_route_weights_backward(const float* logits, const int* topk_idx, const float* grad, int T, int K, float scale,
                                   float* grad_logits, cudaStream_t st) {
-  B200MOE_CUDA_TRY(launch_pdl(k_route_weights_backward, dim3((T + 7) / 8), dim3(256), 0, st, logits, topk_idx, grad, T, K,
+  B200MOE_CUDA_TRY(launch_pdl(k_route_weights_backward,
+                              dim3((T + ROUTE_GRAD_WARPS * ROUTE_GRAD_TOKENS - 1) / (ROUTE_GRAD_WARPS * ROUTE_GRAD_TOKENS)),
+                              dim3(ROUTE_GRAD_WARPS * 32), 0, st, logits, topk_idx, grad, T, K,
                               scale, grad_logits));
   return B200MOE_OK;
 }

@@ -60,8 +60,8 @@ def _backward(grad_y, grad_stream, stream, weight, eps, need_x: bool, need_resid
     T, columns = stream.shape
     device = stream.device
     one = grad_y.dtype is stream.dtype
-    grad_x = grad_y.new_empty((T, columns)) if need_x or (one and need_residual) else None
-    grad_residual = grad_x if one else stream.new_empty((T, columns)) if need_residual else None
+    grad_x = grad_y.new_empty(T, columns) if need_x or (one and need_residual) else None
+    grad_residual = grad_x if one else stream.new_empty(T, columns) if need_residual else None
     grad_weight = None
     if T == 0:
         grad_weight = torch.zeros(columns, dtype=weight.dtype, device=device) if need_weight else None
@@ -69,7 +69,7 @@ def _backward(grad_y, grad_stream, stream, weight, eps, need_x: bool, need_resid
         partial = None
         if need_weight:
             grad_weight = weight.new_empty(columns)
-            partial = weight.new_empty((min(T, _lib.NORM_PARTIAL_ROWS), columns), dtype=torch.float32)
+            partial = weight.new_empty(min(T, _lib.NORM_PARTIAL_ROWS), columns, dtype=torch.float32)
         gy, gy_pitch = row_pointer(grad_y)
         gs, gs_pitch = (None, 0) if grad_stream is None else row_pointer(grad_stream)
         rr, r_pitch = row_pointer(stream)
@@ -88,8 +88,8 @@ def _backward(grad_y, grad_stream, stream, weight, eps, need_x: bool, need_resid
 class _AddRmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps):
-        y = x.new_empty(x.shape)
-        stream = None if residual is None else residual.new_empty(x.shape)
+        y = x.new_empty(*x.shape)
+        stream = None if residual is None else residual.new_empty(*x.shape)
         _forward(x, residual, weight, eps, stream, y, None, None)
         ctx.save_for_backward(x if residual is None else stream, weight)
         ctx.eps, ctx.x_dtype = eps, x.dtype
@@ -125,8 +125,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
         if residual is None:
             return _AddRmsNorm.apply(x, None, weight, eps), x
         return _AddRmsNorm.apply(x, residual, weight, eps)
-    y = x.new_empty((T, columns))
-    stream = x if residual is None else residual.new_empty((T, columns))
+    y = x.new_empty(T, columns)
+    stream = x if residual is None else residual.new_empty(T, columns)
     _forward(x, residual, weight, eps, stream, y, None, None)
     return y, stream
 
@@ -161,7 +161,7 @@ def add_rms_norm_quantize(x: torch.Tensor, residual: Optional[torch.Tensor], wei
             raise ValueError("residual_out needs a residual")
         stream = x
     elif residual_out is None:
-        stream = residual.new_empty((T, columns))
+        stream = residual.new_empty(T, columns)
     else:
         stream = residual_out
         check_tensor(stream, "residual_out", residual.dtype, (T, columns))
@@ -172,9 +172,9 @@ def add_rms_norm_quantize(x: torch.Tensor, residual: Optional[torch.Tensor], wei
             same = t.data_ptr() == stream.data_ptr() and t.dtype is stream.dtype and t.is_contiguous() and t is not weight
             if not same and _overlap(t, stream):
                 raise ValueError(f"residual_out overlaps {name} without being it")
-    q = x.new_empty((T, columns), dtype=_FP8)
-    scale = x.new_empty((columns // QBLOCK, T), dtype=torch.float32)
-    y = x.new_empty((T, columns)) if with_normed else None
+    q = x.new_empty(T, columns, dtype=_FP8)
+    scale = x.new_empty(columns // QBLOCK, T, dtype=torch.float32)
+    y = x.new_empty(T, columns) if with_normed else None
     _forward(x, residual, weight, eps, stream, y, q, scale)
     return (q, scale, stream, y) if with_normed else (q, scale, stream)
 

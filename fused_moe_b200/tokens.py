@@ -81,7 +81,7 @@ def sort_tokens(topk_idx: torch.Tensor, E_local: int, local_expert_offset=0, ali
     need = C.c_size_t(0)
     _lib.check(lib.b200moe_token_sort_scratch_bytes(T, K, E_local, C.byref(need)), "b200moe_token_sort_scratch_bytes")
     ints = topk_idx.new_empty
-    plan = TokenSort(ints(E_local), ints(E_local + 1), ints(rows), ints((T, K)), rows, align)
+    plan = TokenSort(ints(E_local), ints(E_local + 1), ints(rows), ints(T, K), rows, align)
     scratch = ints(need.value // 4) if need.value else None   # a small batch needs none
     with on_device(device):
         _lib.check(lib.b200moe_token_sort(idx.data_ptr(), T, K, E_local, offset, align, rows,
@@ -106,7 +106,7 @@ def _check_batch(t, name: str, plan: TokenSort, rows: int) -> int:
 
 def _gather(x: torch.Tensor, plan_rows: int, row_pairs: torch.Tensor, scatter_map: torch.Tensor) -> torch.Tensor:
     (T, K), columns, device = scatter_map.shape, x.shape[1], x.device
-    out = x.new_empty((plan_rows, columns))
+    out = x.new_empty(plan_rows, columns)
     xr, pitch = row_pointer(x)
     with on_device(device):
         _lib.check(_lib.load().b200moe_token_gather(xr.data_ptr(), pitch, DTYPES[x.dtype], T, K, columns, plan_rows,
@@ -117,7 +117,7 @@ def _gather(x: torch.Tensor, plan_rows: int, row_pairs: torch.Tensor, scatter_ma
 
 def _combine(rows: torch.Tensor, weights: Optional[torch.Tensor], scatter_map: torch.Tensor) -> torch.Tensor:
     (T, K), columns, device = scatter_map.shape, rows.shape[1], rows.device
-    out = rows.new_empty((T, columns))
+    out = rows.new_empty(T, columns)
     rr, pitch = row_pointer(rows)
     w = None if weights is None else dense(weights)
     with on_device(device):
@@ -132,8 +132,8 @@ def _combine(rows: torch.Tensor, weights: Optional[torch.Tensor], scatter_map: t
 def _combine_backward(grad, rows, weights, row_pairs, scatter_map, need_rows: bool, need_weights: bool):
     """``rows`` may be None where the weights' gradient is not needed."""
     (T, K), columns, device, n = scatter_map.shape, grad.shape[1], grad.device, row_pairs.shape[0]
-    grad_rows = grad.new_empty((n, columns)) if need_rows else None
-    grad_weights = weights.new_empty((T, K)) if need_weights else None
+    grad_rows = grad.new_empty(n, columns) if need_rows else None
+    grad_weights = weights.new_empty(T, K) if need_weights else None
     gr, g_pitch = row_pointer(grad)
     rr, r_pitch = (None, 0) if rows is None else row_pointer(rows)
     w = dense(weights)
@@ -234,7 +234,7 @@ def _check_logits(routing_logits, topk_idx) -> tuple:
 
 def _route_weights(logits, idx, scale: float) -> torch.Tensor:
     T, K = idx.shape
-    out = logits.new_empty((T, K))
+    out = logits.new_empty(T, K)
     logits, idx = dense(logits), dense(idx)
     with on_device(logits.device):
         _lib.check(_lib.load().b200moe_route_weights(logits.data_ptr(), idx.data_ptr(), T, K, scale, out.data_ptr(),
@@ -245,7 +245,7 @@ def _route_weights(logits, idx, scale: float) -> torch.Tensor:
 
 def _route_weights_backward(logits, idx, grad, scale: float) -> torch.Tensor:
     T, K = idx.shape
-    out = logits.new_empty((T, E_GLOBAL))
+    out = logits.new_empty(T, E_GLOBAL)
     logits, idx, grad = dense(logits), dense(idx), dense(grad)
     with on_device(logits.device):
         _lib.check(_lib.load().b200moe_route_weights_backward(logits.data_ptr(), idx.data_ptr(), grad.data_ptr(), T, K, scale,

@@ -220,9 +220,9 @@ int b200moe_add_rms_norm(const void* x, int64_t x_pitch, int32_t x_type, const v
                          float eps, void* stream_out, void* y_out, void* q_out, float* scale_out, void* stream);
 /* Its gradient.  grad_y [T, columns] of `type`, grad_stream (optional) and stream_rows = the r of the forward call of stream_type:
  *   dr = (g - r * mean(g * r) / v) / sqrt(v) + grad_stream,   g = grad_y * weight,  v = mean(r^2) + eps
- * grad_x (optional) receives dr in `type`, grad_residual (optional) in stream_type, grad_weight (optional) the sum over tokens of
- * grad_y * r / sqrt(v) in weight_type.  With grad_weight, `partial` is scratch of min(T, B200MOE_NORM_PARTIAL_ROWS) rows
- * of `columns` floats.  Every sum has a fixed order: the same call gives the same bits. */
+ * grad_x (optional) receives dr in `type`, grad_residual (optional) in stream_type, grad_weight (optional) the sum over
+ * tokens of grad_y * r / sqrt(v) in weight_type.  With grad_weight, `partial` is scratch of min(T, B200MOE_NORM_PARTIAL_ROWS)
+ * rows of `columns` floats.  Every sum has a fixed order: the same call gives the same bits. */
 #define B200MOE_NORM_PARTIAL_ROWS 512
 int b200moe_add_rms_norm_backward(const void* grad_y, int64_t grad_y_pitch, int32_t type, const void* grad_stream,
                                   int64_t grad_stream_pitch, const void* stream_rows, int64_t stream_pitch,
@@ -232,8 +232,9 @@ int b200moe_add_rms_norm_backward(const void* grad_y, int64_t grad_y_pitch, int3
 
 /* Tokens sorted by expert, for experts that are the caller's own products (training, other weights than the layer's).
  * topk_idx [T, K], K <= 8: ids outside [offset, offset + E_local) take no part (-1 for the padding of a batch), and a token may
- * name an expert twice.  Pair p = t * K + k gets row offsets[e] + (pairs of expert e before p); every segment starts at a multiple
- * of `align`; a pair whose row would be `rows` (the capacity) or more gets none.  T * K + E_local * (align - 1) and `rows` are at most B200MOE_TOKEN_MAX_ROWS.
+ * name an expert twice.  Pair p = t * K + k gets row offsets[e] + (pairs of expert e before p); every segment starts at a
+ * multiple of `align`; a pair whose row would be `rows` (the capacity) or more gets none.  T * K + E_local * (align - 1) and
+ * `rows` are at most B200MOE_TOKEN_MAX_ROWS.
  *   counts [E_local]       pairs of each local expert, those without a row among them
  *   offsets [E_local + 1]  first row of each segment and the end of the last, at most `rows`
  *   row_pairs [rows]       pair of each row, -1 for a row without one
@@ -250,13 +251,13 @@ int b200moe_token_sort(const int32_t* topk_idx, int32_t T, int32_t K, int32_t E_
 int b200moe_token_gather(const void* x, int64_t x_pitch, int32_t type, int32_t T, int32_t K, int32_t columns, int32_t rows,
                          const int32_t* row_pairs, const int32_t* scatter_map, void* out, void* stream);
 /* out[t] = sum over k of weights[t,k] * rows_in[row(t,k)], k ascending, float32 sums, rounded once; zeros for a token without a row.
- * weights NULL: 1, which is the gradient of b200moe_token_gather.  An entry of a map outside 0 .. rows - 1 counts as -1 in all of
- * these calls. */
+ * weights NULL: 1, which is the gradient of b200moe_token_gather.  An entry of a map outside 0 .. rows - 1 counts as -1 in
+ * all of these calls. */
 int b200moe_token_combine(const void* rows_in, int64_t rows_pitch, int32_t type, const float* weights, int32_t T, int32_t K,
                           int32_t columns, int32_t rows, const int32_t* scatter_map, void* out, void* stream);
 /* Gradient of b200moe_token_combine: grad_rows[row(t,k)] = weights[t,k] * grad[t], zeros in the other rows (optional);
- * grad_weights[t,k] = sum over columns of grad[t] * rows_in[row(t,k)], 0 for a pair without a row (optional; rows_in may be NULL
- * without it). */
+ * grad_weights[t,k] = sum over columns of grad[t] * rows_in[row(t,k)], 0 for a pair without a row (optional; rows_in may be
+ * NULL without it). */
 int b200moe_token_combine_backward(const void* grad, int64_t grad_pitch, const void* rows_in, int64_t rows_pitch,
                                    int32_t type, const float* weights, int32_t T, int32_t K, int32_t columns, int32_t rows,
                                    const int32_t* row_pairs, const int32_t* scatter_map, void* grad_rows,

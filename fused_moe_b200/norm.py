@@ -168,6 +168,8 @@ def add_rms_norm_quantize(x: torch.Tensor, residual: Optional[torch.Tensor], wei
         check_device(x, stream)
         if not stream.is_contiguous() or stream.data_ptr() % 16:
             raise ValueError("residual_out must be contiguous and 16-byte aligned")
+        if stream.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("residual_out is overwritten and must not require a gradient")
         for name, t in (("x", x), ("residual", residual), ("weight", weight)):
             same = t.data_ptr() == stream.data_ptr() and t.dtype is stream.dtype and t.is_contiguous() and t is not weight
             if not same and _overlap(t, stream):
@@ -176,6 +178,8 @@ def add_rms_norm_quantize(x: torch.Tensor, residual: Optional[torch.Tensor], wei
     scale = x.new_empty(columns // QBLOCK, T, dtype=torch.float32)
     y = x.new_empty(T, columns) if with_normed else None
     _forward(x, residual, weight, eps, stream, y, q, scale)
+    if residual_out is not None:
+        torch.autograd.graph.increment_version(residual_out)   # who saved its old values for a gradient learns of the write
     return (q, scale, stream, y) if with_normed else (q, scale, stream)
 
 

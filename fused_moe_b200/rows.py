@@ -104,6 +104,8 @@ def differentiable_once(backward):
         with torch.no_grad():
             results = backward(ctx, *grads)
         results = results if isinstance(results, tuple) else (results,)
+        if all(r is None for r in results):
+            return results
         return _FirstDerivative.apply(torch.empty(0, requires_grad=True), *results)
     return call
 

@@ -60,7 +60,7 @@ def poison(*shapes):
 
 
 SHAPES = [(1, 8), (1, 7168), (2, 128), (3, 200), (7, 512), (5, 2048), (33, 2056), (17, 4096), (4, 4104), (3, 8192), (2, 16384),
-          (333, 7168), (1025, 264)]
+          (333, 7168), (1025, 264), (1030, 7168), (1026, 2056), (1100, 1024), (2000, 576), (70001, 128)]
 TYPES = [(BF16, BF16), (BF16, F32), (BF16, None), (F16, F16), (F16, F32), (F32, F32), (F32, None)]
 
 
@@ -276,6 +276,38 @@ def test_one_tensor_as_x_and_residual(norm):
     got = torch.autograd.grad((y, r), leaf, (gy, gs))[0]
     a, b, _ = norm.add_rms_norm_backward(gy, gs, r.detach(), w)
     assert torch.equal(got, a + b)
+
+
+def test_offsets_past_32_bits(norm):
+    """More than 2^31 elements and 2^32 bytes: the last rows are those of a call on themselves."""
+    T, n = 300_032, 7168
+    x = torch.randn(T, n, device="cuda", dtype=BF16)
+    res = torch.randn(T, n, device="cuda", dtype=BF16)
+    w = torch.randn(n, device="cuda", dtype=BF16)
+    q, s, r, y = norm.add_rms_norm_quantize(x, res, w, with_normed=True)
+    for part in (slice(0, 3), slice(T // 2, T // 2 + 3), slice(T - 3, T)):
+        want = norm.add_rms_norm_quantize(x[part], res[part], w, with_normed=True)
+        assert torch.equal(q[part].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(s[:, part], want[1])
+        assert torch.equal(r[part], want[2]) and torch.equal(y[part], want[3])
+    del q, s, r
+    gx, gr, gw = norm.add_rms_norm_backward(y, x, res, w)
+    for part in (slice(0, 3), slice(T - 3, T)):
+        # another launch shape may add a row's squares in another order: a rounding of the result apart
+        want = grads64(y[part], x[part], res[part], w)
+        assert_within(gx[part], want[0], u(BF16) * want[0].abs() + 2 * ARITH * want[1] + tiny(BF16), "grad")
+    assert gr is gx and gw.isfinite().all()
+
+
+def test_a_destination_counts_the_write(norm):
+    """A tensor that autograd has saved notices that it was overwritten; one that requires a gradient is refused."""
+    x, res, w, _ = make(4, 256, F32, F32, seed=18)
+    leaf = x.clone().requires_grad_()
+    y = leaf * res
+    norm.add_rms_norm_quantize(x, res, w, residual_out=res)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with pytest.raises(RuntimeError, match="must not require"):
+        norm.add_rms_norm_quantize(x, res, w, residual_out=res.clone().requires_grad_())
 
 
 def test_empty_batch(norm):

@@ -274,6 +274,29 @@ def test_rows_of_another_batch_do_no_harm(tok):
     torch.cuda.synchronize()
 
 
+def test_offsets_past_32_bits(tok):
+    """More than 2^31 elements and 2^32 bytes of sorted rows."""
+    T, n = 40_100, 7168
+    idx = select(T, 8, 16)
+    plan = tok.sort_tokens(idx, 256)
+    assert plan.rows * n > 2 ** 31
+    x = torch.randn(T, n, device="cuda", dtype=BF16)
+    xs = tok.gather_tokens(x, plan)
+    pick = torch.tensor([0, 1, plan.rows // 2, plan.rows - 2, plan.rows - 1], device="cuda")
+    assert torch.equal(xs[pick], x[(plan.row_pairs[pick] // 8).long()])
+    w = torch.rand(T, 8, device="cuda")
+    y = tok.combine_tokens(xs, w, plan)
+    some = torch.tensor([0, 7, T // 2, T - 1], device="cuda")
+    want = x[some].double() * w[some].double().sum(dim=1, keepdim=True)
+    assert_within(y[some], want, (u(BF16) + 8 * EPS24) * want.abs() + 8 * EPS24 * want.abs(), "combined")
+    gh, gw = tok.combine_tokens_backward(x, xs, w, plan)
+    pair = plan.row_pairs[pick].long()
+    want = w.flatten()[pair].double()[:, None] * x[pair // 8].double()
+    assert_within(gh[pick], want, (u(BF16) + 2 * EPS24) * want.abs() + tiny(BF16), "grad of rows")
+    dots = x[some].double().square().sum(dim=1, keepdim=True).expand(-1, 8)
+    assert_within(gw[some], dots, (n / 32 + 21) * EPS24 * dots, "grad of weights")
+
+
 def test_empty_batches(tok):
     idx = torch.empty((0, 8), dtype=torch.int32, device="cuda")
     plan = tok.sort_tokens(idx, 32, 64, align=128)

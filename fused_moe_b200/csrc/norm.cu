@@ -335,7 +335,15 @@ static int forward_vpt(int T, int n_vec) { return n_vec > 1024 || (n_vec > 64 &&
 static int backward_vpt(bool wide_stream, int n_vec) {
   return n_vec > 1024 || (n_vec > 512 && !wide_stream) ? 4 : n_vec > 32 ? 2 : 1;
 }
-constexpr int BACKWARD_THREADS = 256;   // of a CTA that works on several tokens at once
+// Tokens that a CTA of the backward kernel works on at once.  More of them leave fewer rows of partial sums to add (us with about
+// 256 / 512 threads per CTA: 8192 x 2048 29.3 / 27.2, 4096 x 7168 45.1 / 42.2, 1000 x 4096 15.2 / 12.5), as long as the SMs are
+// evenly used (333 x 7168 8.4 / 10.3: 84 CTAs with four tokens each) and a small batch has a CTA for each token.
+static int backward_groups(int T, int row_threads, int num_sms) {
+  const int most = MAX_WARPS * 32 / row_threads, half = MAX_WARPS * 16 / row_threads;
+  if (T <= 64) return 1;
+  if (T < 4 * num_sms && (T + most - 1) / most > num_sms) return half > 1 ? half : 1;
+  return most;
+}
 struct NormShape {
   int n_vec, vpt, threads;   // threads: of a row
 };
@@ -401,8 +409,8 @@ int launch_add_rms_norm_backward(const void* grad_y, long long grad_y_pitch, int
     using W = decltype(wt);
     constexpr int VPT = decltype(vpt)::value;
     const size_t stage = static_cast<size_t>(columns) * (sizeof(X) + sizeof(R) * (grad_stream ? 2 : 1));
-    // tokens that a CTA works on at once: about BACKWARD_THREADS threads' worth
-    const int groups = s.threads >= BACKWARD_THREADS ? 1 : BACKWARD_THREADS / s.threads;
+    int groups = backward_groups(T, s.threads, num_sms);
+    while (groups > 1 && 2 * stage * groups > static_cast<size_t>(MAX_DYNAMIC_SMEM)) --groups;
     auto launch = [&](auto stages, auto is_exact) -> int {
       auto kern = k_add_rms_norm_backward<X, R, W, VPT, decltype(stages)::value, decltype(is_exact)::value>;
       const size_t smem = stage * stages * groups;

@@ -289,38 +289,52 @@ k_add_rms_norm_backward(const uint8_t* grad_y, long long grad_y_pitch, const uin
   }
 }
 
-// dweight[c] = sum of the rows of `partial`, rounded once: 32 columns per CTA, its warps take the rows in turn, sixteen in
-// flight.
+// dweight[c] = sum of the rows of `partial`, rounded once: 32 columns per CTA, 16 bytes per lane (four rows a warp and load), all of
+// a thread's loads in flight at once.
 constexpr int WEIGHT_GRAD_WARPS = 16;
 __global__ void __launch_bounds__(WEIGHT_GRAD_WARPS * 32)
 k_norm_weight_grad(const float* partial, int rows, int columns, int type, void* grad_weight) {
-  __shared__ float s[WEIGHT_GRAD_WARPS][32];
+  __shared__ float4 s[WEIGHT_GRAD_WARPS][8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
+  const int c = blockIdx.x * 32 + (lane & 7) * 4;   // `columns` is a multiple of 8: four columns are inside it or outside
+  constexpr int STEP = WEIGHT_GRAD_WARPS * 4, LOADS = B200MOE_NORM_PARTIAL_ROWS / STEP;
+  static_assert(LOADS * STEP == B200MOE_NORM_PARTIAL_ROWS, "whole rounds");
   pdl_launch_dependents();
   pdl_wait();
-  float sum = 0.f;
-  for (int r = warp; c < columns && r < rows; r += 16 * WEIGHT_GRAD_WARPS) {
-    float v[16];
+  float4 v[LOADS], sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int row = r + i * WEIGHT_GRAD_WARPS;
-      v[i] = row < rows ? ld_dep(partial + static_cast<long long>(row) * columns + c) : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sum += v[i];
+  for (int i = 0; i < LOADS; ++i) {
+    const int r = warp * 4 + (lane >> 3) + i * STEP;
+    v[i] = r < rows && c < columns ? ld_dep(reinterpret_cast<const float4*>(partial + static_cast<long long>(r) * columns + c))
+                                   : make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  s[warp][lane] = sum;
-  __syncthreads();
-  if (warp != 0 || c >= columns) return;
 #pragma unroll
-  for (int i = 1; i < WEIGHT_GRAD_WARPS; ++i) sum += s[i][lane];
+  for (int i = 0; i < LOADS; ++i) {
+    sum.x += v[i].x;
+    sum.y += v[i].y;
+    sum.z += v[i].z;
+    sum.w += v[i].w;
+  }
+#pragma unroll
+  for (int d = 8; d <= 16; d <<= 1) {
+    sum.x += __shfl_xor_sync(0xffffffffu, sum.x, d);
+    sum.y += __shfl_xor_sync(0xffffffffu, sum.y, d);
+    sum.z += __shfl_xor_sync(0xffffffffu, sum.z, d);
+    sum.w += __shfl_xor_sync(0xffffffffu, sum.w, d);
+  }
+  if (lane < 8) s[warp][lane] = sum;
+  __syncthreads();
+  const int column = blockIdx.x * 32 + lane;
+  if (warp != 0 || column >= columns) return;
+  float all = 0.f;
+#pragma unroll
+  for (int i = 0; i < WEIGHT_GRAD_WARPS; ++i) all += reinterpret_cast<const float*>(s[i])[lane];
   if (type == B200MOE_DTYPE_F32) {
-    static_cast<float*>(grad_weight)[c] = sum;
+    static_cast<float*>(grad_weight)[column] = all;
   } else if (type == B200MOE_DTYPE_F16) {
-    static_cast<__half*>(grad_weight)[c] = __float2half_rn(sum);
+    static_cast<__half*>(grad_weight)[column] = __float2half_rn(all);
   } else {
-    static_cast<__nv_bfloat16*>(grad_weight)[c] = __float2bfloat16_rn(sum);
+    static_cast<__nv_bfloat16*>(grad_weight)[column] = __float2bfloat16_rn(all);
   }
 }
 

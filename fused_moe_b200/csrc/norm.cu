@@ -15,7 +15,7 @@
 // instruction, predicated vectors and the weight's type looked up at run time issued 31 (forward, e4m3) and 43 (backward) warp
 // instructions per element and lane and ran at 5.5 and 3.7 TB/s; paired operations, types as template arguments and rows of
 // whole vectors brought 16384 x 7168 bf16 to 124 us with e4m3 out (826 MB: 6.6 TB/s; 132 - 139 in a long run, where the
-// clocks settle lower), 137 us with bf16 out (940 MB) and 146 us backward (940 MB and the partial sums).
+// clocks settle lower), 137 us with bf16 out (940 MB) and 142 us backward (940 MB and the partial sums).
 #include <type_traits>
 
 #include "row_vec.cuh"

@@ -218,6 +218,38 @@ def test_gradients_against_differences(tok):
         assert abs((grad.double() * d).sum() - diff) <= 40 * EPS24 * size * 8
 
 
+def test_what_lies_in_masked_places_is_not_used(tok):
+    """NaN and infinities in the weights and gradients of pairs without a row, in rows without a pair and in the logits of experts
+    that no pair names leave no trace."""
+    T, n = 50, 136
+    idx = select(T, 8, 17, "padded")
+    g = torch.Generator(device="cuda").manual_seed(21)
+    rnd = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    plan = tok.sort_tokens(idx, 128, 64, align=16, rows=100)
+    has, used = plan.scatter_map >= 0, plan.row_pairs >= 0
+    assert not has.all() and not used.all() and has.any()
+    x, h, w, gy, gxs = rnd(T, n), rnd(100, n), rnd(T, 8), rnd(T, n), rnd(100, n)
+    idle = ~has.any(dim=1)   # tokens without any row
+    assert idle.any()
+
+    def results(x, h, w, gy, gxs):
+        return (tok.gather_tokens(x, plan), tok.combine_tokens(h, w, plan), tok.gather_tokens_backward(gxs, plan),
+                *tok.combine_tokens_backward(gy, h, w, plan))
+
+    want = results(x, h, w, gy, gxs)
+    for bad in (float("nan"), float("inf"), -3.4e38):
+        x2, h2, w2, gy2, gxs2 = (t.clone() for t in (x, h, w, gy, gxs))
+        x2[idle], gy2[idle], h2[~used], gxs2[~used], w2[~has] = bad, bad, bad, bad, bad
+        assert all(torch.equal(a, b) for a, b in zip(results(x2, h2, w2, gy2, gxs2), want))
+    logits, gw = rnd(T, 256), rnd(T, 8)
+    want = tok.route_weights(logits, idx, 2.5), tok.route_weights_backward(logits, idx, gw, 2.5)
+    named = torch.zeros((T, 257), dtype=torch.bool, device="cuda").scatter_(1, torch.where(idx >= 0, idx, 256).long(), True)
+    for bad in (float("nan"), float("inf"), -3.4e38):
+        l2, gw2 = torch.where(named[:, :256], logits, bad), torch.where(idx >= 0, gw, bad)
+        assert torch.equal(tok.route_weights(l2, idx, 2.5), want[0])
+        assert torch.equal(tok.route_weights_backward(l2, idx, gw2, 2.5), want[1])
+
+
 def test_partial_gradients(tok):
     idx = select(20, 8, 9)
     plan = tok.sort_tokens(idx, 256)

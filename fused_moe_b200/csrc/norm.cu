@@ -7,9 +7,11 @@
 //
 // Backward, with g = dy * weight and n = H columns:
 //   dr = rstd * (g - r * rstd^2 * mean(g * r)) + dr_out       dweight = sum over tokens of dy * r * rstd
-// rstd is recomputed: sum(r^2) and sum(g * r) are taken in the same pass over the row.
+// rstd is recomputed: sum(r^2) and sum(g * r) are taken in the same pass over the row.  The second term is taken as
+// (r * rstd) * (rstd * (rstd * mean(g * r))): the first factor is of order 1 and the second of the gradient's own size, so neither
+// leaves float32 where the result does not (rstd^3 does, for rows of magnitude 1e14 or 1e-13), and dy * (r * rstd) likewise.
 //
-// Sums and statistics are float32.
+// Sums and statistics are float32: the squares of a row have to add up to less than 3.4e38 (elements of 1e17 do at 7168 columns).
 //
 // Bound by the bytes of the rows once the instructions are out of the way: a first form with one float32 operation per
 // instruction, predicated vectors and the weight's type looked up at run time issued 31 (forward, e4m3) and 43 (backward) warp
@@ -236,7 +238,7 @@ k_add_rms_norm_backward(const uint8_t* grad_y, long long grad_y_pitch, const uin
     const float n = static_cast<float>(n_vec * 8);
     const float rstd1 = __frsqrt_rn(__shfl_sync(0xffffffffu, half, 0) / n + eps);
     const float mean = __shfl_sync(0xffffffffu, half, 16) / n;
-    const float2 rstd = both(rstd1), c = both(-(rstd1 * rstd1 * rstd1 * mean));
+    const float2 rstd = both(rstd1), c = both(-(rstd1 * (rstd1 * mean)));
     const long long row = static_cast<long long>(t) * n_vec;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -251,9 +253,9 @@ k_add_rms_norm_backward(const uint8_t* grad_y, long long grad_y_pitch, const uin
       if (grad_stream) unpack_vec8<R>(shared_vec8<R>(slot + n_vec * (PX + PR), v), d);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        g[j] = mul2(g[j], rstd);
+        r[j] = mul2(r[j], rstd);
         acc[i][j] = fma2(g[j], r[j], acc[i][j]);
-        d[j] = fma2(g[j], w[j], fma2(r[j], c, d[j]));
+        d[j] = fma2(mul2(g[j], rstd), w[j], fma2(r[j], c, d[j]));
       }
       if (grad_x) store_vec8<X>(grad_x + row * 8 * sizeof(X), v, pack_vec8<X>(d));
       if (grad_residual) store_vec8<R>(grad_residual + row * 8 * sizeof(R), v, pack_vec8<R>(d));

@@ -3,7 +3,9 @@
 ``add_rms_norm_quantize`` goes from the residual stream to the ``hidden_states`` / ``hidden_states_scale`` pair that
 ``kernel`` takes in one launch; ``add_rms_norm`` is the same norm for training, differentiable in all three inputs.  Both follow
   r = x + residual, rounded to the residual's type        y = r * weight / sqrt(mean(r^2) + eps)
-with float32 arithmetic on the rounded r.  The reference takes quantised activations as given and has no such operator.
+with float32 arithmetic on the rounded r.  The squares of a row have to stay in float32's range: above about 1e17 per element
+their sum is infinite and y is 0; under 1e-19 they are 0, which is nothing beside an ordinary eps, but leaves ``eps=0`` without
+a norm.  The reference takes quantised activations as given and has no such operator.
 """
 from __future__ import annotations
 

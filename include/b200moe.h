@@ -209,7 +209,7 @@ int b200moe_quantize_act(const void* x_bf16, int32_t T, void* q_out, float* scal
 
 /* Residual addition and RMS norm, with the layer's quantisation on the way out:
  *   r = x + residual, rounded to residual_type          (residual NULL: r = x, stream_out is not written)
- *   y = r * weight / sqrt(mean(r^2) + eps)              float32 arithmetic on the rounded r
+ *   y = r * weight / sqrt(mean(r^2) + eps)              float32 arithmetic on the rounded r, whose sum of squares must fit
  * stream_out [T, columns] of residual_type receives r (it may be `residual` itself); y_out (optional) y in x_type; q_out and
  * scale_out (optional, together) e4m3 rows and their float32 scales [columns / 128, T] by the rule of b200moe_quantize_act,
  * applied to the float32 y; a NaN in a block makes its scale NaN.

@@ -420,3 +420,43 @@ def test_second_derivatives_are_refused(norm):
     assert torch.equal(g, norm.add_rms_norm_backward(torch.ones_like(y), None, (x + res).detach(), w)[0])
     with pytest.raises(RuntimeError, match="differentiable once"):
         (g.sum() + x.square().sum()).backward()
+
+
+@pytest.mark.parametrize("dtype, stream, scale, grad_scale, eps", [
+    (F32, F32, 1e14, 1.0, EPS), (F32, F32, 1e15, 1.0, EPS), (F32, F32, 1e16, 1.0, EPS), (F32, F32, 1e16, 1e-8, EPS),
+    (F32, None, 1e-18, 1.0, EPS), (F32, F32, 1e-13, 1.0, 0.0), (F32, None, 1e-16, 1e-3, 0.0), (BF16, BF16, 1e16, 1.0, EPS),
+    (BF16, F32, 1e15, 1.0, EPS), (BF16, BF16, 1e-13, 1.0, 0.0), (BF16, BF16, 1e4, 1.0, EPS), (BF16, None, 1e-4, 1.0, EPS),
+    (F16, F16, 100.0, 1.0, EPS), (F16, F16, 1e-3, 1.0, EPS)], ids=str)
+@pytest.mark.parametrize("T, n", [(9, 2048), (3, 264), (200, 1024)])
+def test_backward_of_large_and_small_rows(norm, T, n, dtype, stream, scale, grad_scale, eps):
+    """Rows far from magnitude 1, with gradients that have a component along the row, so that both terms of the gradient count.
+    No factor leaves the type's range where the result does not.  Rounding errors, in units of 2^-24 of the terms' magnitudes:
+    a sum over a row is at most 16 terms in a thread's chain and 10 levels of the tree, once whole for mean(g r) and twice
+    half for 1 / sqrt; with the products, divisions and roots at most 64, which is 2^-18."""
+    x, res, w, rnd = make(T, n, dtype, stream, seed=20, scale=scale)
+    r, _ = ref64(x, res, w, eps)
+    unit = r.double() / r.double().square().mean(dim=1, keepdim=True).sqrt()
+    gy = (grad_scale * (rnd(T, n) + 0.5 * unit)).to(dtype)
+    gs = None if stream is None else (grad_scale * rnd(T, n) / (3 * scale)).to(stream)
+    if dtype is F16:
+        gs = None   # of the size of the rest of the gradient, it would leave the type's range
+    grads = norm.add_rms_norm_backward(gy, gs, r, w, eps)
+    dr, size, dw, dw_size = grads64(gy, gs, r, w, eps)
+    assert dr.abs().max() > 0.1 * size.max()
+    for got in grads[:2]:
+        assert got.isfinite().all()
+        assert_within(got, dr, u(got.dtype) * dr.abs() + 2.0 ** -18 * size + tiny(got.dtype), "grad of x or residual")
+    chain = (T / 148 + 73) * 2.0 ** -24
+    assert_within(grads[2], dw, u(w.dtype) * dw.abs() + (ARITH + chain) * dw_size + tiny(w.dtype), "grad of weight")
+
+
+@pytest.mark.parametrize("dtype, eps", [(F32, 1e-26), (F32, 1e-30), (BF16, 1e-30), (F32, 1e-36)], ids=str)
+def test_backward_of_a_row_of_zeros(norm, dtype, eps):
+    """dr = g / sqrt(eps), also where eps^(-3/2) would leave float32."""
+    r = torch.zeros((3, 512), dtype=dtype, device="cuda")
+    r[1] = torch.randn(512, device="cuda").to(dtype)
+    gy, w = torch.randn(3, 512, device="cuda").to(dtype), torch.ones(512, dtype=dtype, device="cuda")
+    got = norm.add_rms_norm_backward(gy, None, r, w, eps)
+    dr, size, dw, dw_size = grads64(gy, None, r, w, eps)
+    assert_within(got[0], dr, u(dtype) * dr.abs() + 2.0 ** -18 * size, "grad of x")
+    assert_within(got[2], dw, u(dtype) * dw.abs() + 2.0 ** -18 * dw_size, "grad of weight")

@@ -92,15 +92,32 @@ def sort_tokens(topk_idx: torch.Tensor, E_local: int, local_expert_offset=0, ali
     return plan
 
 
-def _check_batch(t, name: str, plan: TokenSort, rows: int) -> int:
+def _check_plan(plan) -> TokenSort:
+    """A plan may have been put together by hand or from several: the arrays that the kernels index are checked on every call.
+    (Their entries are not read here; the kernels take one that lies outside the buffers for -1.)"""
     if not isinstance(plan, TokenSort):
         raise TypeError("plan must be a TokenSort")
+    scatter_map, row_pairs = plan.scatter_map, plan.row_pairs
+    for t, name in ((scatter_map, "scatter_map"), (row_pairs, "row_pairs")):
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32:
+            raise TypeError(f"plan.{name} must be an int32 tensor")
+        if not t.is_contiguous():
+            raise ValueError(f"plan.{name} must be contiguous")
+    if scatter_map.dim() != 2 or not 1 <= scatter_map.shape[1] <= TOP_K or scatter_map.shape[0] > MAX_TOKENS:
+        raise ValueError(f"plan.scatter_map must be [T, K] with K in 1..{TOP_K} and T <= {MAX_TOKENS}, got "
+                         f"{tuple(scatter_map.shape)}")
+    if row_pairs.shape != (plan.rows,):
+        raise ValueError(f"plan.row_pairs must have plan.rows = {plan.rows} entries, got {tuple(row_pairs.shape)}")
+    return plan
+
+
+def _check_batch(t, name: str, plan: TokenSort, rows: int) -> int:
     n, columns = check_rows(t, name)
     if n != rows:
         raise ValueError(f"{name} must have {rows} rows, got {n}")
     if columns == 0 or columns * t.element_size() % 16 or columns > 1 << 24:
         raise ValueError(f"a row of {name} must be a multiple of 16 bytes, got {columns} columns of {t.dtype}")
-    check_device(t, plan.scatter_map)
+    check_device(t, plan.scatter_map, plan.row_pairs)
     return columns
 
 
@@ -178,8 +195,7 @@ def gather_tokens(x: torch.Tensor, plan: TokenSort) -> torch.Tensor:
     """[plan.rows, n]: row r is x[t] for the pair (t, k) of row r, and zero for a row without a pair.  x [T, n] bf16, f16 or f32 with
     rows of whole 16 bytes; row-strided input is read in place.  Differentiable once in x: the gradient of a token is the sum
     of its rows' gradients, in float32, in the order of k."""
-    if not isinstance(plan, TokenSort):
-        raise TypeError("plan must be a TokenSort")
+    _check_plan(plan)
     _check_batch(x, "x", plan, plan.scatter_map.shape[0])
     if records_graph("gather_tokens_backward", x):
         return _GatherTokens.apply(x, plan)
@@ -188,8 +204,7 @@ def gather_tokens(x: torch.Tensor, plan: TokenSort) -> torch.Tensor:
 
 def gather_tokens_backward(grad: torch.Tensor, plan: TokenSort) -> torch.Tensor:
     """Gradient [T, n] of the x of ``gather_tokens`` from that of its result; can be captured into a CUDA graph."""
-    if not isinstance(plan, TokenSort):
-        raise TypeError("plan must be a TokenSort")
+    _check_plan(plan)
     _check_batch(grad, "grad", plan, plan.rows)
     return _combine(grad, None, plan.scatter_map)
 
@@ -204,8 +219,7 @@ def combine_tokens(rows: torch.Tensor, topk_weights: torch.Tensor, plan: TokenSo
     type of ``rows``; zero for a token without a row.  rows [plan.rows, n] bf16, f16 or f32, topk_weights [T, K] f32.
     Rows without a pair are not read.  Differentiable once in both: rows without a pair get gradient 0, so do the weights of
     pairs without a row."""
-    if not isinstance(plan, TokenSort):
-        raise TypeError("plan must be a TokenSort")
+    _check_plan(plan)
     _check_batch(rows, "rows", plan, plan.rows)
     _check_weights(topk_weights, plan, rows)
     if records_graph("combine_tokens_backward", rows, topk_weights):
@@ -216,8 +230,7 @@ def combine_tokens(rows: torch.Tensor, topk_weights: torch.Tensor, plan: TokenSo
 def combine_tokens_backward(grad: torch.Tensor, rows: torch.Tensor, topk_weights: torch.Tensor, plan: TokenSort):
     """Gradients (grad_rows, grad_weights) of ``combine_tokens`` from that of its result, in one pass over the rows; can be
     captured into a CUDA graph."""
-    if not isinstance(plan, TokenSort):
-        raise TypeError("plan must be a TokenSort")
+    _check_plan(plan)
     _check_batch(grad, "grad", plan, plan.scatter_map.shape[0])
     check_tensor(rows, "rows", grad.dtype, (plan.rows, grad.shape[1]))
     check_device(grad, rows)

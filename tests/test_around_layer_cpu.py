@@ -255,3 +255,48 @@ def test_constants_match_the_header():
     assert value("B200MOE_NORM_MAX_COLUMNS") == _lib.NORM_MAX_COLUMNS
     assert value("B200MOE_NORM_PARTIAL_ROWS") == _lib.NORM_PARTIAL_ROWS
     assert value("B200MOE_TOKEN_MAX_ROWS") == _lib.TOKEN_MAX_ROWS
+
+
+def _plan_calls(p):
+    """Every call that takes a plan, on tensors that pass for CUDA ones and fit three tokens and 24 rows."""
+    x, h, w = (_cuda_like(t) for t in (rows(), rows(T=24), torch.zeros((3, 8))))
+    return (lambda: tokens.gather_tokens(x, p), lambda: tokens.gather_tokens_backward(h, p), lambda: tokens.combine_tokens(h, w, p),
+            lambda: tokens.combine_tokens_backward(x, h, w, p))
+
+
+def _ints(*shape, dtype=torch.int32):
+    return _cuda_like(torch.zeros(shape, dtype=dtype))
+
+
+@pytest.mark.parametrize("error, match, change", [
+    (ValueError, "plan.rows", lambda: dict(row_pairs=_ints(23))),                    # shorter than the capacity: read past its end
+    (ValueError, "plan.rows", lambda: dict(row_pairs=_ints(25))),
+    (ValueError, "plan.rows", lambda: dict(row_pairs=_ints(24, 1))),
+    (ValueError, "contiguous", lambda: dict(row_pairs=_ints(48)[::2])),
+    (TypeError, "row_pairs", lambda: dict(row_pairs=_ints(24, dtype=torch.int64))),
+    (TypeError, "row_pairs", lambda: dict(row_pairs=None)),
+    (ValueError, "contiguous", lambda: dict(scatter_map=_ints(8, 3).t())),
+    (ValueError, "contiguous", lambda: dict(scatter_map=_ints(3, 16)[:, ::2])),
+    (TypeError, "scatter_map", lambda: dict(scatter_map=_ints(3, 8, dtype=torch.int64))),
+    (TypeError, "scatter_map", lambda: dict(scatter_map=_ints(3, 8, dtype=torch.float32))),
+    (TypeError, "scatter_map", lambda: dict(scatter_map=[[0] * 8] * 3)),
+    (ValueError, "scatter_map", lambda: dict(scatter_map=_ints(24))),
+    (ValueError, "scatter_map", lambda: dict(scatter_map=_ints(3, 9))),
+    (ValueError, "scatter_map", lambda: dict(scatter_map=_ints(3, 0))),
+    (RuntimeError, "CUDA|device", lambda: dict(row_pairs=torch.zeros(24, dtype=torch.int32))),
+    (RuntimeError, "CUDA|device", lambda: dict(scatter_map=torch.zeros((3, 8), dtype=torch.int32))),
+], ids=range(16))
+@pytest.mark.parametrize("which", range(4))
+def test_plans_whose_arrays_do_not_fit_are_refused(which, error, match, change):
+    """A plan is a public tuple: its arrays may come from anywhere."""
+    with pytest.raises(error, match=match):
+        _plan_calls(_cuda_plan()._replace(**change()))[which]()
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_a_plan_with_a_larger_capacity_than_its_arrays_is_refused(which):
+    p = _cuda_plan()._replace(rows=1000)
+    x, h, w = (_cuda_like(t) for t in (rows(), rows(T=1000), torch.zeros((3, 8))))
+    with pytest.raises(ValueError, match="plan.rows"):
+        (lambda: tokens.gather_tokens(x, p), lambda: tokens.gather_tokens_backward(h, p), lambda: tokens.combine_tokens(h, w, p),
+         lambda: tokens.combine_tokens_backward(x, h, w, p))[which]()

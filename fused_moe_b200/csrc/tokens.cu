@@ -7,8 +7,9 @@
 //   gather    out[row(t,k)] = x[t]                    backward: grad_x[t] = sum_k grad[row(t,k)]    (= combine, weights 1)
 //   combine   out[t] = sum_k w[t,k] * in[row(t,k)]    backward: grad_in[row(t,k)] = w[t,k] * grad[t]
 //                                                               grad_w[t,k] = sum over columns of grad[t] * in[row(t,k)]
-// Rows without a pair are written as zeros.  The kernels walk tokens, not rows: a token's row is read once and written to (or
-// summed from) its at most eight rows.  No atomics on values, every sum in a fixed order; sums are float32.
+// Rows without a pair, and rows whose pair the map sends elsewhere, are written as zeros.  The kernels walk tokens, not rows: a
+// token's row is read once and written to (or summed from) its at most eight rows.  No atomics on values, every sum in a fixed
+// order; sums are float32.
 #include "route_token.cuh"
 #include "row_vec.cuh"
 
@@ -168,31 +169,48 @@ __device__ __forceinline__ TokenPairs token_pairs(const int* scatter_map, const 
   return p;
 }
 
-// CTA i's share of the rows (grid.x CTAs; at most 32 rows each, checked by the host) is looked through for rows without a pair,
-// which become zeros in the pieces [begin, end) of this CTA.
-__device__ __forceinline__ void zero_unused_rows(const int* row_pairs, int rows, uint8_t* out, int pieces, int begin, int end) {
-  const int lane = threadIdx.x & 31;
-  const int first = static_cast<int>(static_cast<long long>(rows) * blockIdx.x / gridDim.x);
-  const int last = static_cast<int>(static_cast<long long>(rows) * (blockIdx.x + 1) / gridDim.x);
-  uint32_t unused = __ballot_sync(0xffffffffu, first + lane < last && ld_dep(row_pairs + min(first + lane, rows - 1)) < 0);
-  for (; unused; unused &= unused - 1) {
-    uint4* dst = reinterpret_cast<uint4*>(out) + static_cast<long long>(first + __ffs(unused) - 1) * pieces;
+// CTA i's share of the rows are the `per` rows from i * per on (at most 32: rows_per_cta()), one per lane of every warp; -1: none.
+__device__ __forceinline__ int share_row(int per, int rows) {
+  const int lane = threadIdx.x & 31, row = blockIdx.x * per + lane;
+  return lane < per && row < rows ? row : -1;
+}
+__device__ __forceinline__ int share_pair(const int* row_pairs, int per, int rows) {
+  const int row = share_row(per, rows);
+  return row >= 0 ? ld_dep(row_pairs + row) : -1;
+}
+// The row that the map names for a pair, -1 for what is none of the batch's pairs.  Where that is not the row that names the
+// pair, no token writes the row.
+__device__ __forceinline__ int named_row(const int* scatter_map, int pair, int n_pairs) {
+  return static_cast<uint32_t>(pair) < static_cast<uint32_t>(n_pairs) ? ld_dep(scatter_map + pair) : -1;
+}
+// The rows of the share that no token writes become zeros in the pieces [begin, end).
+__device__ __forceinline__ void zero_unused_rows(int named, int per, int rows, uint8_t* out, int pieces, int begin, int end) {
+  const int mine = share_row(per, rows);
+  for (uint32_t unused = __ballot_sync(0xffffffffu, mine >= 0 && named != mine); unused; unused &= unused - 1) {
+    const int row = blockIdx.x * per + __ffs(unused) - 1;
+    uint4* dst = reinterpret_cast<uint4*>(out) + static_cast<long long>(row) * pieces;
     for (int p = begin + threadIdx.x; p < end; p += blockDim.x) dst[p] = make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
 // out[row(t,k)] = x[t]; CTA (t, y) copies the y-th part of the token's row, and zeroes its share of the unused rows.  Bound
-// by its stores, which do not stay in L2 (streaming: 171 -> 169 us): 8192 tokens x 8 rows of 7168 bf16 are 1.06 GB, 6.3 TB/s.
+// by its stores, which do not stay in L2 (streaming: 171 -> 169 us): 8192 tokens x 8 rows of 7168 bf16 are 1.06 GB in 170 us,
+// 6.2 TB/s.
 constexpr int TOKEN_UNROLL = 4;   // pieces of a row in flight per thread
 __global__ void __launch_bounds__(256)
-k_token_gather(const uint8_t* x, long long x_pitch, int T, int K, int rows, int pieces, const int* row_pairs,
+k_token_gather(const uint8_t* x, long long x_pitch, int T, int K, int rows, int per, int pieces, const int* row_pairs,
                const int* scatter_map, uint8_t* out) {
   pdl_launch_dependents();
   pdl_wait();
   const int t = blockIdx.x;
   const int part = (pieces + gridDim.y - 1) / gridDim.y, begin = blockIdx.y * part, end = min(begin + part, pieces);
+  // the share's two loads depend on one another: one ahead of those of the token's pairs and one behind, so that nothing waits for
+  // either (1 token 2.2 us, 64 tokens 4.2; both behind the token's work 2.3 and 4.5)
+  const int pair = share_pair(row_pairs, per, rows);
+  TokenPairs pairs = {-1, 1.f, 0u};
+  if (t < T) pairs = token_pairs(scatter_map, nullptr, t, K, rows);
+  const int named = named_row(scatter_map, pair, T * K);
   if (t < T) {
-    const TokenPairs pairs = token_pairs(scatter_map, nullptr, t, K, rows);
     const uint4* src = reinterpret_cast<const uint4*>(x + t * x_pitch);
     for (int p0 = begin + threadIdx.x; pairs.mask && p0 - static_cast<int>(threadIdx.x) < end; p0 += TOKEN_UNROLL * blockDim.x) {
       uint4 v[TOKEN_UNROLL];
@@ -208,7 +226,7 @@ k_token_gather(const uint8_t* x, long long x_pitch, int T, int K, int rows, int 
       }
     }
   }
-  zero_unused_rows(row_pairs, rows, out, pieces, begin, end);
+  zero_unused_rows(named, per, rows, out, pieces, begin, end);
 }
 
 // The rows of up to N pairs of a token, in the order of k: the lowest N bits of the mask.
@@ -279,7 +297,7 @@ k_token_combine(const uint8_t* in, long long in_pitch, const float* weights, int
     combine_rows<X, TOP_K, 1>(in, in_pitch, pairs, begin, end, dst);
 }
 
-// One pass over the rows gives both gradients: 8192 tokens x 8 rows of 7168 bf16 are 2.0 GB in 303 us, 6.6 TB/s.
+// One pass over the rows gives both gradients: 8192 tokens x 8 rows of 7168 bf16 are 2.0 GB in 305 us, 6.5 TB/s.
 //
 // grad_in[row(t,k)] = w[t,k] * grad[t] and the token's dot products <grad[t], in[row(t,k)]>, summed over the CTA into
 // s_dot[j][warp] for the j-th pair with a row; N and U as for combine_rows.
@@ -344,7 +362,7 @@ __device__ __forceinline__ void combine_rows_backward(const uint4* grad, const u
 template <typename X, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
 k_token_combine_backward(const uint8_t* grad, long long grad_pitch, const uint8_t* in, long long in_pitch,
-                         const float* weights, int T, int K, int rows, int pieces, const int* row_pairs,
+                         const float* weights, int T, int K, int rows, int per, int pieces, const int* row_pairs,
                          const int* scatter_map, uint8_t* grad_in, float* grad_w) {
   __shared__ float s_dot[TOP_K][16];
   pdl_launch_dependents();
@@ -368,7 +386,12 @@ k_token_combine_backward(const uint8_t* grad, long long grad_pitch, const uint8_
       }
     }
   }
-  if (grad_in) zero_unused_rows(row_pairs, rows, grad_in, pieces, 0, pieces);
+  if (grad_in) {
+    // behind the token's work: registers are what this kernel is short of (loaded ahead of it 311 us at 8192 tokens x 8 rows of
+    // 7168 bf16, here 305.5; f16, which spills 20 bytes, 310)
+    const int named = named_row(scatter_map, share_pair(row_pairs, per, rows), T * K);
+    zero_unused_rows(named, per, rows, grad_in, pieces, 0, pieces);
+  }
 }
 
 // w[t,k] = scale * s_k / (sum_j s_j + 1e-20) over the token's K selected experts, s = sigmoid(logit): the operations, and their
@@ -476,11 +499,13 @@ int launch_token_sort(const int* topk_idx, int T, int K, int E_local, int offset
   return B200MOE_OK;
 }
 
-// One CTA per token, more where the capacity has many rows per token: at most nine rows per CTA to look through.
+// One CTA per token, more where the capacity has many rows per token.
 static unsigned token_ctas(int T, int rows) {
   const int by_rows = (rows + TOP_K - 1) / TOP_K;
   return static_cast<unsigned>(T > by_rows ? T : by_rows);
 }
+// Rows that each of them looks through: at most nine.
+static int rows_per_cta(int rows, unsigned ctas) { return static_cast<int>((rows + static_cast<long long>(ctas) - 1) / ctas); }
 static unsigned token_threads(int pieces, int most) {
   const int threads = (pieces + 31) / 32 * 32;
   return static_cast<unsigned>(threads < most ? threads : most);
@@ -499,8 +524,8 @@ int launch_token_gather(const void* x, long long x_pitch, int T, int K, int rows
                         const int* scatter_map, void* out, cudaStream_t st) {
   const unsigned ctas = token_ctas(T, rows), threads = token_threads(pieces, 256);
   B200MOE_CUDA_TRY(launch_pdl(k_token_gather, dim3(ctas, token_parts(ctas, pieces, threads)), dim3(threads), 0, st,
-                              static_cast<const uint8_t*>(x), x_pitch, T, K, rows, pieces, row_pairs, scatter_map,
-                              static_cast<uint8_t*>(out)));
+                              static_cast<const uint8_t*>(x), x_pitch, T, K, rows, rows_per_cta(rows, ctas), pieces, row_pairs,
+                              scatter_map, static_cast<uint8_t*>(out)));
   return B200MOE_OK;
 }
 
@@ -529,9 +554,10 @@ int launch_token_combine_backward(const void* grad, long long grad_pitch, const 
     using X = decltype(xt);
     const bool few = T <= 148;
     auto kern = few ? k_token_combine_backward<X, 512> : k_token_combine_backward<X, 256>;
-    B200MOE_CUDA_TRY(launch_pdl(kern, dim3(grad_in ? token_ctas(T, rows) : T), dim3(token_threads(pieces, few ? 512 : 256)),
-                                0, st, static_cast<const uint8_t*>(grad), grad_pitch, static_cast<const uint8_t*>(in),
-                                in_pitch, weights, T, K, rows, pieces, row_pairs, scatter_map,
+    const unsigned ctas = grad_in ? token_ctas(T, rows) : static_cast<unsigned>(T);
+    B200MOE_CUDA_TRY(launch_pdl(kern, dim3(ctas), dim3(token_threads(pieces, few ? 512 : 256)), 0, st,
+                                static_cast<const uint8_t*>(grad), grad_pitch, static_cast<const uint8_t*>(in), in_pitch,
+                                weights, T, K, rows, rows_per_cta(rows, ctas), pieces, row_pairs, scatter_map,
                                 static_cast<uint8_t*>(grad_in), grad_w));
     return B200MOE_OK;
   });

@@ -247,7 +247,9 @@ int b200moe_token_sort_scratch_bytes(int32_t T, int32_t K, int32_t E_local, size
 int b200moe_token_sort(const int32_t* topk_idx, int32_t T, int32_t K, int32_t E_local, int32_t offset, int32_t align,
                        int32_t rows, void* scratch, size_t scratch_bytes, int32_t* counts, int32_t* offsets,
                        int32_t* row_pairs, int32_t* scatter_map, void* stream);
-/* out[row(t,k)] = x[t] for every pair with a row; the other rows become zeros.  columns * element size: a multiple of 16. */
+/* out[row(t,k)] = x[t] for every pair with a row; the other rows become zeros.  row_pairs and scatter_map are those of one sort, from
+ * which pairs may have been taken out since: a row whose entry is none of the batch's pairs, or a pair that scatter_map
+ * sends elsewhere, is one without a pair.  No two pairs have one row.  columns * element size: a multiple of 16. */
 int b200moe_token_gather(const void* x, int64_t x_pitch, int32_t type, int32_t T, int32_t K, int32_t columns, int32_t rows,
                          const int32_t* row_pairs, const int32_t* scatter_map, void* out, void* stream);
 /* out[t] = sum over k of weights[t,k] * rows_in[row(t,k)], k ascending, float32 sums, rounded once; zeros for a token without a row.

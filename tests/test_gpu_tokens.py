@@ -557,3 +557,43 @@ def test_training_block(tok):
     for name, a, b in zip(("out", "x", "res", "w", "gate", "experts"), got, want):
         rel = ((a.double() - b).norm() / b.norm()).item()
         assert rel <= 1.5e-3, (name, rel)
+
+
+@pytest.mark.parametrize("T, n, align, K", [(10, 64, 1, 8), (200, 520, 16, 8), (700, 2048, 1, 3)])
+def test_rows_whose_pair_has_lost_them_are_zeros(tok, T, n, align, K):
+    """A map that has been edited behind the sort (pairs dropped with -1, entries outside the
+    buffers): the rows that no pair names any more are zeros, like all rows without a pair."""
+    idx = select(T, K, 30, "uniform")
+    plan = tok.sort_tokens(idx, 256, align=align)
+    R = plan.rows
+    g = torch.Generator(device="cuda").manual_seed(22)
+    x, gy = torch.randn(T, n, generator=g, device="cuda"), torch.randn(T, n, generator=g, device="cuda")
+    h, w = torch.randn(R, n, generator=g, device="cuda"), torch.randn(T, K, generator=g, device="cuda")
+    edited = plan.scatter_map.clone()
+    edited[::3, 0], edited[1::3, 1], edited[2::3, 2] = -1, R, -2 ** 31
+    named = torch.zeros(R, dtype=torch.bool, device="cuda")
+    named[edited[(edited >= 0) & (edited < R)].long()] = True
+    full = tok.gather_tokens(x, plan), tok.combine_tokens_backward(gy, h, w, plan)[0]
+    for pairs in (plan.row_pairs, plan.row_pairs.clone().fill_(2 ** 31 - 1)):
+        plan2 = plan._replace(scatter_map=edited, row_pairs=pairs)
+        if pairs is not plan.row_pairs:   # pairs that are none of the batch's: no row is anybody's
+            plan2 = plan2._replace(scatter_map=torch.full_like(edited, -1))
+            named = torch.zeros_like(named)
+        poison(R, n, F32)
+        xs = tok.gather_tokens(x, plan2)
+        assert torch.equal(xs, torch.where(named[:, None], full[0], 0.0))
+        poison(R, n, F32)
+        gh, gw = tok.combine_tokens_backward(gy, h, w, plan2)
+        assert torch.equal(gh, torch.where(named[:, None], full[1], 0.0))
+        assert gw[(plan2.scatter_map < 0) | (plan2.scatter_map >= R)].eq(0).all()
+
+
+def test_rows_of_a_larger_batch_are_zeros(tok):
+    """row_pairs of a batch with more tokens: pairs behind the batch's own are none of it."""
+    big, small = tok.sort_tokens(select(40, 8, 31), 256), tok.sort_tokens(select(20, 8, 32), 256, rows=320)
+    x = torch.randn(20, 64, device="cuda")
+    behind = (big.row_pairs >= 160) & ~torch.isin(torch.arange(320, device="cuda", dtype=torch.int32), small.scatter_map.flatten())
+    assert behind.any()
+    poison(320, 64, F32)
+    xs = tok.gather_tokens(x, small._replace(row_pairs=big.row_pairs))
+    assert xs[behind].eq(0).all()

@@ -7,6 +7,7 @@ import functools
 from typing import Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .kernel import _require_cuda
@@ -36,8 +37,19 @@ def check_tensor(t, name: str, dtype: torch.dtype, shape: Tuple[int, ...]) -> No
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
 
 
+def refuse_tangents(*tensors) -> None:
+    """Forward-mode derivatives are not available: a tensor that carries a tangent (it need not require a gradient) would come out
+    without one, which counts as zero.  Outside of ``forward_ad.dual_level()`` there are none."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("the operators around the layer have no forward-mode derivative: an input carries a tangent")
+
+
 def check_device(first: torch.Tensor, *tensors) -> torch.device:
-    """The CUDA device of ``first``, on which all others must be too."""
+    """The CUDA device of ``first``, on which all others must be too.  Every operator passes all its tensors through here, so tangents
+    are refused here as well."""
     device = first.device
     for t in tensors:
         if t is not None and t.device != device:
@@ -45,6 +57,7 @@ def check_device(first: torch.Tensor, *tensors) -> torch.device:
             raise RuntimeError(f"all tensors must live on one device: got {t.device} beside {device}")
     if not first.is_cuda:
         _require_cuda(input=first)
+    refuse_tangents(first, *tensors)
     return device
 
 
@@ -99,6 +112,7 @@ def differentiable_once(backward):
     require one; the results of a constant gradient would count as constants of the inputs.)"""
     @functools.wraps(backward)
     def call(ctx, *grads):
+        refuse_tangents(*grads)
         if not torch.is_grad_enabled():
             return backward(ctx, *grads)
         with torch.no_grad():

@@ -300,3 +300,60 @@ def test_a_plan_with_a_larger_capacity_than_its_arrays_is_refused(which):
     with pytest.raises(ValueError, match="plan.rows"):
         (lambda: tokens.gather_tokens(x, p), lambda: tokens.gather_tokens_backward(h, p), lambda: tokens.combine_tokens(h, w, p),
          lambda: tokens.combine_tokens_backward(x, h, w, p))[which]()
+
+
+# ---- derivatives that an operator does not have -------------------------------------------------------------------------------
+def _operators():
+    """(call on a dict of tensors, names of its tensors that have a derivative); on tensors that pass for CUDA ones."""
+    t = {k: _cuda_like(v) for k, v in dict(
+        x=rows(), res=rows(), w=torch.ones(256), h=rows(T=24), tw=torch.zeros((3, 8)), logits=torch.zeros((3, 256)),
+        gy=rows(), gs=rows(), gl=torch.zeros((3, 8))).items()}
+    p, i = _cuda_plan(), _cuda_like(ids())
+    return t, {
+        "add_rms_norm": (lambda a: norm.add_rms_norm(a["x"], a["res"], a["w"]), ("x", "res", "w")),
+        "first norm": (lambda a: norm.add_rms_norm(a["x"], None, a["w"]), ("x", "w")),
+        "add_rms_norm_backward": (lambda a: norm.add_rms_norm_backward(a["gy"], a["gs"], a["res"], a["w"]), ("gy", "gs", "res", "w")),
+        "add_rms_norm_quantize": (lambda a: norm.add_rms_norm_quantize(a["x"], a["res"], a["w"]), ("x", "res", "w")),
+        "gather_tokens": (lambda a: tokens.gather_tokens(a["x"], p), ("x",)),
+        "gather_tokens_backward": (lambda a: tokens.gather_tokens_backward(a["h"], p), ("h",)),
+        "combine_tokens": (lambda a: tokens.combine_tokens(a["h"], a["tw"], p), ("h", "tw")),
+        "combine_tokens_backward": (lambda a: tokens.combine_tokens_backward(a["x"], a["h"], a["tw"], p), ("x", "h", "tw")),
+        "route_weights": (lambda a: tokens.route_weights(a["logits"], i, 2.5), ("logits",)),
+        "route_weights_backward": (lambda a: tokens.route_weights_backward(a["logits"], i, a["gl"], 2.5), ("logits", "gl"))}
+
+
+@pytest.mark.parametrize("name", list(_operators()[1]))
+def test_tangents_are_refused(name):
+    """A dual tensor does not require a gradient; its tangent must not get lost."""
+    from torch.autograd import forward_ad
+    t, calls = _operators()
+    call, names = calls[name]
+    for which in names:
+        with forward_ad.dual_level():
+            dual = _cuda_like(forward_ad.make_dual(t[which].as_subclass(torch.Tensor), torch.ones(t[which].shape, dtype=t[which].dtype)))
+            assert not dual.requires_grad and forward_ad.unpack_dual(dual).tangent is not None
+            with pytest.raises(RuntimeError, match="carries a tangent"):
+                call(t | {which: dual})
+
+
+def test_tangents_of_incoming_gradients_are_refused():
+    """Forward over reverse: the gradient of the result carries the tangent, the inputs do not."""
+    from torch.autograd import forward_ad
+    from fused_moe_b200.rows import differentiable_once
+
+    class Double(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return 2 * x
+
+        @staticmethod
+        @differentiable_once
+        def backward(ctx, g):
+            return g.detach() * 2
+
+    x = torch.zeros(3, requires_grad=True)
+    y = Double.apply(x)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="carries a tangent"):
+            torch.autograd.grad(y, x, forward_ad.make_dual(torch.ones(3), torch.ones(3)), retain_graph=True)
+    assert torch.autograd.grad(y, x, torch.ones(3))[0].eq(2).all()

@@ -155,9 +155,15 @@ def add_rms_norm_quantize(x: torch.Tensor, residual: Optional[torch.Tensor], wei
     q [T, n] e4m3 and scales [n / 128, T] float32 are the ``hidden_states`` / ``hidden_states_scale`` of ``kernel`` (n = 7168), by
     the rule of ``quantize_activations`` on the float32 y; r is the residual stream after the addition; y the normalised rows in
     the type of ``x``, which the router's product reads.  Arguments as for ``add_rms_norm`` with n a multiple of 128.
-    ``residual_out`` [T, n] of the residual's type receives r and may be ``residual`` itself."""
+    ``residual_out`` [T, n] of the residual's type receives r and may be ``residual`` itself.  Not differentiable: with gradients
+    enabled, an input that requires one is refused."""
     T, columns = _check(x, residual, weight, eps, QBLOCK)
     check_device(x, residual, weight)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
+        # r is the residual stream that the rest of the model builds on: without a graph, everything below it would stay without
+        # a gradient
+        raise RuntimeError("add_rms_norm_quantize is not differentiable: call it under torch.no_grad(), or add_rms_norm for "
+                           "gradients")
     if residual is None:
         if residual_out is not None:
             raise ValueError("residual_out needs a residual")

@@ -357,3 +357,23 @@ def test_tangents_of_incoming_gradients_are_refused():
         with pytest.raises(RuntimeError, match="carries a tangent"):
             torch.autograd.grad(y, x, forward_ad.make_dual(torch.ones(3), torch.ones(3)), retain_graph=True)
     assert torch.autograd.grad(y, x, torch.ones(3))[0].eq(2).all()
+
+
+@pytest.mark.parametrize("which", ["x", "res", "w"])
+@pytest.mark.parametrize("residual", [True, False])
+def test_the_quantised_norm_refuses_to_drop_a_gradient(monkeypatch, which, residual):
+    t, _ = _operators()
+    if which == "res" and not residual:
+        return
+    leaf = t[which].clone().requires_grad_()
+    a = t | {which: _cuda_like(leaf) if not isinstance(leaf, _Fake) else leaf}
+    call = lambda: norm.add_rms_norm_quantize(a["x"], a["res"] if residual else None, a["w"])  # noqa: E731
+    assert a[which].requires_grad
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        call()
+    launched = []
+    monkeypatch.setattr(norm, "_forward", lambda *args: launched.append(args))   # no launch from these tensors, wherever this runs
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            call()
+    assert len(launched) == 2

@@ -20,7 +20,7 @@ import torch
 from . import _lib
 from .kernel import E_GLOBAL, TOP_K, _host_scalar
 from .rows import DTYPES, MAX_TOKENS, check_device, check_rows, check_tensor, dense, differentiable_once, on_device, \
-    records_graph, refuse_capture, row_pointer, stream_of
+    records_graph, refuse_capture, refuse_tangents, row_pointer, stream_of
 
 
 class TokenSort(NamedTuple):
@@ -282,14 +282,24 @@ class _RouteWeights(torch.autograd.Function):
         return _route_weights_backward(*ctx.saved_tensors, grad, ctx.scale), None, None
 
 
+def _scale(x) -> float:
+    """``routed_scaling_factor`` as a number.  A tensor's own derivative is not computed and must not get lost."""
+    if torch.is_tensor(x):
+        refuse_tangents(x)
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("routed_scaling_factor has no gradient here: pass a number or a detached tensor")
+    return _host_scalar(x, float)
+
+
 def route_weights(routing_logits: torch.Tensor, topk_idx: torch.Tensor, routed_scaling_factor) -> torch.Tensor:
     """[T, K] float32: the weights s_k / (sum_j s_j + 1e-20) * routed_scaling_factor, s = sigmoid(logit), of the experts that
     ``topk_idx`` [T, K] int32 (K <= 8) names; for the selection of ``kernel.route`` these are its weights, bit for bit.  Ids
     outside 0..255 (-1 for the padding of a batch) have weight 0 and take no part; a NaN logit makes its token's weights NaN
     (``route`` takes it for a large one).  Differentiable once in the logits [T, 256]
-    float32; the selection itself, and the bias that shaped it, have no gradient."""
+    float32; the selection itself, and the bias that shaped it, have no gradient, and a scaling factor that requires one is
+    refused."""
     _check_logits(routing_logits, topk_idx)
-    scale = _host_scalar(routed_scaling_factor, float)
+    scale = _scale(routed_scaling_factor)
     if records_graph("route_weights_backward", routing_logits):
         return _RouteWeights.apply(routing_logits, topk_idx, scale)
     return _route_weights(routing_logits, topk_idx, scale)
@@ -301,4 +311,4 @@ def route_weights_backward(routing_logits: torch.Tensor, topk_idx: torch.Tensor,
     T, K = _check_logits(routing_logits, topk_idx)
     check_tensor(grad_weights, "grad_weights", torch.float32, (T, K))
     check_device(routing_logits, grad_weights)
-    return _route_weights_backward(routing_logits, topk_idx, grad_weights, _host_scalar(routed_scaling_factor, float))
+    return _route_weights_backward(routing_logits, topk_idx, grad_weights, _scale(routed_scaling_factor))

@@ -377,3 +377,23 @@ def test_the_quantised_norm_refuses_to_drop_a_gradient(monkeypatch, which, resid
         with mode():
             call()
     assert len(launched) == 2
+
+
+def test_a_scaling_factor_that_requires_a_gradient_is_refused(monkeypatch):
+    from torch.autograd import forward_ad
+    t, _ = _operators()
+    i, scale = _cuda_like(ids()), torch.tensor(2.5, requires_grad=True)
+    calls = (lambda s: tokens.route_weights(t["logits"], i, s), lambda s: tokens.route_weights_backward(t["logits"], i, t["gl"], s))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="routed_scaling_factor has no gradient"):
+            call(scale)
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="carries a tangent"):
+            call(forward_ad.make_dual(scale.detach(), torch.tensor(1.0)))
+    seen = []
+    monkeypatch.setattr(tokens, "_route_weights", lambda logits, idx, s: seen.append(s))
+    monkeypatch.setattr(tokens, "_route_weights_backward", lambda logits, idx, grad, s: seen.append(s))
+    for call in calls:
+        call(scale.detach())
+        with torch.no_grad():
+            call(scale)
+    assert seen == [2.5] * 4

@@ -30,15 +30,15 @@ int launch_gemv1(const b200moe_problem*, const b200moe_workspace*, int, cudaStre
 int launch_route_gemv1(const b200moe_problem*, const b200moe_workspace*, int, cudaStream_t);
 int launch_gemv2(const b200moe_problem*, const b200moe_workspace*, int, cudaStream_t);
 int launch_add_rms_norm(const void*, long long, int, const void*, long long, int, const void*, int, int, int, float, void*,
-                        void*, void*, float*, int, cudaStream_t);
+                        void*, void*, float*, cudaStream_t);
 int launch_add_rms_norm_backward(const void*, long long, int, const void*, long long, const void*, long long, int, const void*,
                                  int, int, int, float, void*, void*, void*, float*, int, cudaStream_t);
 size_t token_sort_scratch_bytes(int, int, int);
 int launch_token_sort(const int*, int, int, int, int, int, int, int*, int*, int*, int*, int*, cudaStream_t);
-int launch_token_gather(const void*, long long, int, int, int, int, const int*, const int*, void*, cudaStream_t);
-int launch_token_combine(const void*, long long, int, const float*, int, int, int, int, const int*, void*, cudaStream_t);
+int launch_token_gather(const void*, long long, int, int, int, int, const int*, const int*, void*, int, cudaStream_t);
+int launch_token_combine(const void*, long long, int, const float*, int, int, int, int, const int*, void*, int, cudaStream_t);
 int launch_token_combine_backward(const void*, long long, const void*, long long, int, const float*, int, int, int, int,
-                                  const int*, const int*, void*, float*, cudaStream_t);
+                                  const int*, const int*, void*, float*, int, cudaStream_t);
 int launch_route_weights(const float*, const int*, int, int, float, float*, cudaStream_t);
 int launch_route_weights_backward(const float*, const int*, const float*, int, int, float, float*, cudaStream_t);
 
@@ -233,7 +233,7 @@ int b200moe_add_rms_norm(const void* x, int64_t x_pitch, int32_t x_type, const v
   if ((rc = device_info(&sms))) return rc;
   return launch_add_rms_norm(x, pitch_of(x_pitch, columns, x_type), x_type, residual,
                              pitch_of(residual_pitch, columns, residual_type), residual_type, weight, weight_type, T, columns,
-                             eps, stream_out, y_out, q_out, scale_out, sms, static_cast<cudaStream_t>(stream));
+                             eps, stream_out, y_out, q_out, scale_out, static_cast<cudaStream_t>(stream));
 }
 
 int b200moe_add_rms_norm_backward(const void* grad_y, int64_t grad_y_pitch, int32_t type, const void* grad_stream,
@@ -301,7 +301,7 @@ int b200moe_token_gather(const void* x, int64_t x_pitch, int32_t type, int32_t T
   if (!row_pairs || !out || (T > 0 && (!x || !scatter_map)) || !aligned16(x) || !aligned16(out)) return B200MOE_EINVAL;
   int sms, rc;
   if ((rc = device_info(&sms))) return rc;
-  return launch_token_gather(x, pitch_of(x_pitch, columns, type), T, K, rows, pieces, row_pairs, scatter_map, out,
+  return launch_token_gather(x, pitch_of(x_pitch, columns, type), T, K, rows, pieces, row_pairs, scatter_map, out, sms,
                              static_cast<cudaStream_t>(stream));
 }
 
@@ -315,7 +315,7 @@ int b200moe_token_combine(const void* rows_in, int64_t rows_pitch, int32_t type,
   int sms, rc;
   if ((rc = device_info(&sms))) return rc;
   return launch_token_combine(rows_in, pitch_of(rows_pitch, columns, type), type, weights, T, K, rows, pieces, scatter_map,
-                              out, static_cast<cudaStream_t>(stream));
+                              out, sms, static_cast<cudaStream_t>(stream));
 }
 
 int b200moe_token_combine_backward(const void* grad, int64_t grad_pitch, const void* rows_in, int64_t rows_pitch,
@@ -335,7 +335,7 @@ int b200moe_token_combine_backward(const void* grad, int64_t grad_pitch, const v
   if ((rc = device_info(&sms))) return rc;
   return launch_token_combine_backward(grad, pitch_of(grad_pitch, columns, type), rows_in,
                                        pitch_of(rows_pitch, columns, type), type, weights, T, K, rows, pieces, row_pairs,
-                                       scatter_map, grad_rows, grad_weights, static_cast<cudaStream_t>(stream));
+                                       scatter_map, grad_rows, grad_weights, sms, static_cast<cudaStream_t>(stream));
 }
 
 int b200moe_route_weights(const float* logits, const int32_t* topk_idx, int32_t T, int32_t K, float scale, float* weights,

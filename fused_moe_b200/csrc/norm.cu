@@ -395,7 +395,7 @@ static int with_types(int x_type, int stream_type, int weight_type, int vpt, F&&
 
 int launch_add_rms_norm(const void* x, long long x_pitch, int x_type, const void* residual, long long residual_pitch,
                         int residual_type, const void* weight, int weight_type, int T, int columns, float eps,
-                        void* stream_out, void* y, void* q, float* scale, int num_sms, cudaStream_t st) {
+                        void* stream_out, void* y, void* q, float* scale, cudaStream_t st) {
   const NormShape s = norm_shape(columns, forward_vpt(T, columns / 8));
   return with_types(x_type, residual ? residual_type : x_type, weight_type, s.vpt,
                     [&](auto xt, auto rt, auto wt, auto vpt) -> int {

@@ -513,17 +513,17 @@ static unsigned token_threads(int pieces, int most) {
 // Parts of a row, a CTA each, while the batch alone does not fill the GPU: a call of few tokens is as long as a thread's
 // chain of loads and stores.  us with one CTA per token / with parts, at 7168 bf16 columns: gather of 1 token 3.9 / 2.3, of
 // 333 tokens 14.8 / 8.1; combine 3.1 / 1.6 and 6.1 / 5.0.  (Twice as many parts: 333 tokens 7.6 and 5.8.)
-constexpr unsigned TOKEN_FILL_CTAS = 592;   // four per SM
-static unsigned token_parts(unsigned ctas, int pieces, unsigned threads) {
+constexpr unsigned TOKEN_FILL_CTAS = 4;   // per SM
+static unsigned token_parts(unsigned ctas, int pieces, unsigned threads, int num_sms) {
   const unsigned most = (pieces + threads - 1) / threads;
-  const unsigned want = (TOKEN_FILL_CTAS + ctas - 1) / ctas;
+  const unsigned want = (TOKEN_FILL_CTAS * num_sms + ctas - 1) / ctas;
   return want < most ? want : most;
 }
 
 int launch_token_gather(const void* x, long long x_pitch, int T, int K, int rows, int pieces, const int* row_pairs,
-                        const int* scatter_map, void* out, cudaStream_t st) {
+                        const int* scatter_map, void* out, int num_sms, cudaStream_t st) {
   const unsigned ctas = token_ctas(T, rows), threads = token_threads(pieces, 256);
-  B200MOE_CUDA_TRY(launch_pdl(k_token_gather, dim3(ctas, token_parts(ctas, pieces, threads)), dim3(threads), 0, st,
+  B200MOE_CUDA_TRY(launch_pdl(k_token_gather, dim3(ctas, token_parts(ctas, pieces, threads, num_sms)), dim3(threads), 0, st,
                               static_cast<const uint8_t*>(x), x_pitch, T, K, rows, rows_per_cta(rows, ctas), pieces, row_pairs,
                               scatter_map, static_cast<uint8_t*>(out)));
   return B200MOE_OK;
@@ -537,10 +537,11 @@ static int with_row_type(int type, F&& f) {
 }
 
 int launch_token_combine(const void* in, long long in_pitch, int type, const float* weights, int T, int K, int rows,
-                         int pieces, const int* scatter_map, void* out, cudaStream_t st) {
+                         int pieces, const int* scatter_map, void* out, int num_sms, cudaStream_t st) {
   return with_row_type(type, [&](auto xt) -> int {
     const unsigned threads = token_threads(pieces, 256);
-    B200MOE_CUDA_TRY(launch_pdl(k_token_combine<decltype(xt)>, dim3(T, token_parts(T, pieces, threads)), dim3(threads), 0, st,
+    const unsigned parts = token_parts(T, pieces, threads, num_sms);
+    B200MOE_CUDA_TRY(launch_pdl(k_token_combine<decltype(xt)>, dim3(T, parts), dim3(threads), 0, st,
                                 static_cast<const uint8_t*>(in), in_pitch, weights, K, rows, pieces, scatter_map,
                                 static_cast<uint8_t*>(out)));
     return B200MOE_OK;
@@ -549,10 +550,11 @@ int launch_token_combine(const void* in, long long in_pitch, int type, const flo
 
 int launch_token_combine_backward(const void* grad, long long grad_pitch, const void* in, long long in_pitch, int type,
                                   const float* weights, int T, int K, int rows, int pieces, const int* row_pairs,
-                                  const int* scatter_map, void* grad_in, float* grad_w, cudaStream_t st) {
+                                  const int* scatter_map, void* grad_in, float* grad_w, int num_sms,
+                                  cudaStream_t st) {
   return with_row_type(type, [&](auto xt) -> int {
     using X = decltype(xt);
-    const bool few = T <= 148;
+    const bool few = T <= num_sms;
     auto kern = few ? k_token_combine_backward<X, 512> : k_token_combine_backward<X, 256>;
     const unsigned ctas = grad_in ? token_ctas(T, rows) : static_cast<unsigned>(T);
     B200MOE_CUDA_TRY(launch_pdl(kern, dim3(ctas), dim3(token_threads(pieces, few ? 512 : 256)), 0, st,

@@ -397,3 +397,12 @@ def test_a_scaling_factor_that_requires_a_gradient_is_refused(monkeypatch):
         with torch.no_grad():
             call(scale)
     assert seen == [2.5] * 4
+
+
+def test_the_number_of_multiprocessors_is_the_devices():
+    """No launch rule has one GPU's count of SMs (148, or four CTAs on each, 592) written into it."""
+    import re
+    from conftest import ROOT
+    for name in ("norm.cu", "tokens.cu"):
+        code = re.sub(r"//[^\n]*", "", (ROOT / "fused_moe_b200" / "csrc" / name).read_text())
+        assert not re.search(r"\b(148|296|444|592)\b", code), name

@@ -159,9 +159,9 @@ def add_rms_norm_quantize(x: torch.Tensor, residual: Optional[torch.Tensor], wei
     enabled, an input that requires one is refused."""
     T, columns = _check(x, residual, weight, eps, QBLOCK)
     check_device(x, residual, weight)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
+    if T and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
         # r is the residual stream that the rest of the model builds on: without a graph, everything below it would stay without
-        # a gradient
+        # a gradient.  (An empty batch has none to lose.)
         raise RuntimeError("add_rms_norm_quantize is not differentiable: call it under torch.no_grad(), or add_rms_norm for "
                            "gradients")
     if residual is None:

@@ -377,6 +377,8 @@ def test_the_quantised_norm_refuses_to_drop_a_gradient(monkeypatch, which, resid
         with mode():
             call()
     assert len(launched) == 2
+    empty = {k: _cuda_like(v[:0].detach().clone().requires_grad_()) if k in ("x", "res") else v for k, v in t.items()}
+    norm.add_rms_norm_quantize(empty["x"], empty["res"] if residual else None, empty["w"])   # has no gradient to lose
 
 
 def test_a_scaling_factor_that_requires_a_gradient_is_refused(monkeypatch):

@@ -137,6 +137,8 @@ def records_graph(instead: str, *tensors) -> bool:
 
 
 def refuse_capture(instead: str, device: torch.device) -> None:
+    """Raises if the device's current stream is being captured.  In a backward pass that is the stream of the forward call: autograd
+    makes it current while it runs the node."""
     with on_device(device):
         capturing = torch.cuda.is_current_stream_capturing()
     if capturing:

@@ -597,3 +597,33 @@ def test_rows_of_a_larger_batch_are_zeros(tok):
     poison(320, 64, F32)
     xs = tok.gather_tokens(x, small._replace(row_pairs=big.row_pairs))
     assert xs[behind].eq(0).all()
+
+
+def test_every_backward_pass_asks_for_a_capture_first(tok, monkeypatch):
+    """Under capture autograd's backward passes are refused before they launch anything: each of the four asks, and names the
+    explicit function that is there instead."""
+    from fused_moe_b200 import norm
+
+    class Asked(RuntimeError):
+        pass
+
+    def ask(instead, device):
+        raise Asked(f"{instead} {device.type}")
+
+    idx = select(6, 8, 33)
+    plan = tok.sort_tokens(idx, 256)
+    x, h, w, logits, res, weight = (torch.randn(s, device="cuda").requires_grad_()
+                                    for s in ((6, 64), (48, 64), (6, 8), (6, 256), (6, 64), (64,)))
+    y, r = norm.add_rms_norm(x, res, weight)
+    outs = ((y, "add_rms_norm_backward"), (r, "add_rms_norm_backward"), (norm.add_rms_norm(x, None, weight)[0], "add_rms_norm_backward"),
+            (tok.gather_tokens(x, plan), "gather_tokens_backward"), (tok.combine_tokens(h, w, plan), "combine_tokens_backward"),
+            (tok.route_weights(logits, idx, 2.5), "route_weights_backward"))
+    with monkeypatch.context() as m:
+        m.setattr(norm, "refuse_capture", ask)
+        m.setattr(tok, "refuse_capture", ask)
+        for out, name in outs:
+            with pytest.raises(Asked, match=name + " cuda"):
+                out.sum().backward(retain_graph=True)
+    for out, _ in outs:   # and without a capture they run (y and r are of one node)
+        out.sum().backward(retain_graph=True)
+    assert all(t.grad is not None and t.grad.isfinite().all() for t in (x, h, w, logits, res, weight))

@@ -119,7 +119,9 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
 
     x [T, n] bf16, f16 or f32, n a multiple of 8 up to 16384 · residual [T, n] and weight [n] each of x's type or
     f32.  Row-strided inputs are read in place.  Differentiable once in x, residual and weight; the backward pass saves r and
-    the weight only, and its sums have a fixed order.  During stream capture a call that would record a gradient is
+    the weight only, and its sums have a fixed order: the same call gives the same bits.  A token's results do not depend on
+    its neighbours, but y may differ in its last bit between a batch of at most 1024 tokens and a larger one (rows of 520 to 8192
+    columns: the squares are added by another number of threads).  During stream capture a call that would record a gradient is
     refused (``add_rms_norm_backward`` is the explicit form)."""
     T, columns = _check(x, residual, weight, eps, 8)
     check_device(x, residual, weight)
@@ -154,12 +156,14 @@ def add_rms_norm_quantize(x: torch.Tensor, residual: Optional[torch.Tensor], wei
 
     q [T, n] e4m3 and scales [n / 128, T] float32 are the ``hidden_states`` / ``hidden_states_scale`` of ``kernel`` (n = 7168), by
     the rule of ``quantize_activations`` on the float32 y; r is the residual stream after the addition; y the normalised rows in
-    the type of ``x``, which the router's product reads.  Arguments as for ``add_rms_norm`` with n a multiple of 128.
+    the type of ``x``, which the router's product reads.  Between batches of at most 1024 tokens and larger ones a scale may differ
+    in its last bit, and so a value at the border of two e4m3 steps by one of them.  Arguments as for ``add_rms_norm`` with n a multiple of 128.
     ``residual_out`` [T, n] of the residual's type receives r and may be ``residual`` itself.  Not differentiable: with gradients
     enabled, an input that requires one is refused."""
     T, columns = _check(x, residual, weight, eps, QBLOCK)
     check_device(x, residual, weight)
-    if T and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
+    if (T and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad))
+            and torch.is_grad_enabled()):
         # r is the residual stream that the rest of the model builds on: without a graph, everything below it would stay without
         # a gradient.  (An empty batch has none to lose.)
         raise RuntimeError("add_rms_norm_quantize is not differentiable: call it under torch.no_grad(), or add_rms_norm for "

@@ -92,23 +92,23 @@ def sort_tokens(topk_idx: torch.Tensor, E_local: int, local_expert_offset=0, ali
     return plan
 
 
-def _check_plan(plan) -> TokenSort:
+def _check_plan(plan) -> None:
     """A plan may have been put together by hand or from several: the arrays that the kernels index are checked on every call.
     (Their entries are not read here; the kernels take one that lies outside the buffers for -1.)"""
     if not isinstance(plan, TokenSort):
         raise TypeError("plan must be a TokenSort")
     scatter_map, row_pairs = plan.scatter_map, plan.row_pairs
-    for t, name in ((scatter_map, "scatter_map"), (row_pairs, "row_pairs")):
-        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32:
-            raise TypeError(f"plan.{name} must be an int32 tensor")
-        if not t.is_contiguous():
-            raise ValueError(f"plan.{name} must be contiguous")
-    if scatter_map.dim() != 2 or not 1 <= scatter_map.shape[1] <= TOP_K or scatter_map.shape[0] > MAX_TOKENS:
-        raise ValueError(f"plan.scatter_map must be [T, K] with K in 1..{TOP_K} and T <= {MAX_TOKENS}, got "
-                         f"{tuple(scatter_map.shape)}")
+    if not isinstance(scatter_map, torch.Tensor) or scatter_map.dtype is not torch.int32:
+        raise TypeError("plan.scatter_map must be an int32 tensor")
+    if not isinstance(row_pairs, torch.Tensor) or row_pairs.dtype is not torch.int32:
+        raise TypeError("plan.row_pairs must be an int32 tensor")
+    if not (scatter_map.is_contiguous() and row_pairs.is_contiguous()):
+        raise ValueError("plan.scatter_map and plan.row_pairs must be contiguous")
+    shape = scatter_map.shape
+    if len(shape) != 2 or not 1 <= shape[1] <= TOP_K or shape[0] > MAX_TOKENS:
+        raise ValueError(f"plan.scatter_map must be [T, K] with K in 1..{TOP_K} and T <= {MAX_TOKENS}, got {tuple(shape)}")
     if row_pairs.shape != (plan.rows,):
         raise ValueError(f"plan.row_pairs must have plan.rows = {plan.rows} entries, got {tuple(row_pairs.shape)}")
-    return plan
 
 
 def _check_batch(t, name: str, plan: TokenSort, rows: int) -> int:
@@ -229,7 +229,8 @@ def combine_tokens(rows: torch.Tensor, topk_weights: torch.Tensor, plan: TokenSo
 
 def combine_tokens_backward(grad: torch.Tensor, rows: torch.Tensor, topk_weights: torch.Tensor, plan: TokenSort):
     """Gradients (grad_rows, grad_weights) of ``combine_tokens`` from that of its result, in one pass over the rows; can be
-    captured into a CUDA graph."""
+    captured into a CUDA graph.  The same call gives the same bits; grad_weights may differ in its last ones between a batch of at
+    most as many tokens as the GPU has SMs and a larger one (more threads share a row's sum)."""
     _check_plan(plan)
     _check_batch(grad, "grad", plan, plan.scatter_map.shape[0])
     check_tensor(rows, "rows", grad.dtype, (plan.rows, grad.shape[1]))

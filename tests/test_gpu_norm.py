@@ -460,3 +460,25 @@ def test_backward_of_a_row_of_zeros(norm, dtype, eps):
     dr, size, dw, dw_size = grads64(gy, None, r, w, eps)
     assert_within(got[0], dr, u(dtype) * dr.abs() + 2.0 ** -18 * size, "grad of x")
     assert_within(got[2], dw, u(dtype) * dw.abs() + 2.0 ** -18 * dw_size, "grad of weight")
+
+
+@pytest.mark.parametrize("dtype, stream", [(BF16, BF16), (BF16, F32), (F32, F32)], ids=str)
+@pytest.mark.parametrize("n", [128, 512, 2048, 7168, 8320])
+def test_a_tokens_results_do_not_depend_on_its_neighbours(norm, n, dtype, stream):
+    """Bit for bit: the forward among batches of up to 1024 tokens and among larger ones (and, for rows of at most 512 columns or more
+    than 8192, across the two), the gradient of a row in any batch."""
+    x, res, w, rnd = make(2500, n, dtype, stream, seed=23)
+    gy, gs = rnd(2500, n).to(dtype), rnd(2500, n).to(stream)
+
+    def forward(T):
+        q, s, r, y = norm.add_rms_norm_quantize(x[:T], res[:T], w, with_normed=True)
+        return q.view(torch.uint8), s.t(), r, y
+
+    small, large = {T: forward(T) for T in (1, 5, 333, 1024)}, {T: forward(T) for T in (1025, 2500)}
+    for group in (small, large) if 512 < n <= 8192 else (small | large,):
+        most = max(group)
+        for T, got in group.items():
+            assert all(torch.equal(a, b[:T]) for a, b in zip(got, group[most])), (T, most)
+    back = {T: norm.add_rms_norm_backward(gy[:T], gs[:T], res[:T], w)[:2] for T in (1, 64, 65, 333, 1100, 2500)}
+    for T, got in back.items():
+        assert all(torch.equal(a, b[:T]) for a, b in zip(got, back[2500])), T

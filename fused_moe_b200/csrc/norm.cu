@@ -8,16 +8,18 @@
 // Backward, with g = dy * weight and n = H columns:
 //   dr = rstd * (g - r * rstd^2 * mean(g * r)) + dr_out       dweight = sum over tokens of dy * r * rstd
 // rstd is recomputed: sum(r^2) and sum(g * r) are taken in the same pass over the row.  The second term is taken as
-// (r * rstd) * (rstd * (rstd * mean(g * r))): the first factor is of order 1 and the second of the gradient's own size, so neither
-// leaves float32 where the result does not (rstd^3 does, for rows of magnitude 1e14 or 1e-13), and dy * (r * rstd) likewise.
+// (r * rstd) * (rstd * (rstd * mean(g * r))): the first factor is of order 1 and the second of the gradient's own size, so
+// neither leaves float32 where the result does not (rstd^3 does, for rows of magnitude 1e14 or 1e-13), and dy * (r * rstd)
+// likewise.
 //
-// Sums and statistics are float32: the squares of a row have to add up to less than 3.4e38 (elements of 1e17 do at 7168 columns).
+// Sums and statistics are float32: the squares of a row have to add up to less than 3.4e38 (elements of 1e17 do at 7168
+// columns).
 //
 // Bound by the bytes of the rows once the instructions are out of the way: a first form with one float32 operation per
 // instruction, predicated vectors and the weight's type looked up at run time issued 31 (forward, e4m3) and 43 (backward) warp
 // instructions per element and lane and ran at 5.5 and 3.7 TB/s; paired operations, types as template arguments and rows of
 // whole vectors brought 16384 x 7168 bf16 to 124 us with e4m3 out (826 MB: 6.6 TB/s; 132 - 139 in a long run, where the
-// clocks settle lower), 137 us with bf16 out (940 MB) and 142 us backward (940 MB and the partial sums).
+// clocks settle lower), 137 us with bf16 out (940 MB) and 144 us backward (940 MB and the partial sums).
 #include <type_traits>
 
 #include "row_vec.cuh"
@@ -154,8 +156,10 @@ k_add_rms_norm(const uint8_t* x, long long x_pitch, const uint8_t* residual, lon
 // The rows of a group's next STAGES - 1 tokens are under way in shared memory (16-byte asynchronous copies) while one is worked
 // on: a row's two passes (sums, then output) have a sum over its threads between them, in which nothing would be loaded
 // otherwise.  A thread copies exactly the pieces that it reads itself, so its own wait orders them and the pipeline needs no
-// barrier.  Two stages; a third costs the second CTA per SM (16384 x 7168 bf16: 289 us against 209, when the rest was slower).
-// One where two do not fit into shared memory: float32 rows of more than 9642 columns.
+// barrier.  Two stages (a third, measured with one token per CTA before the rest was faster, cost the second CTA per SM:
+// 16384 x 7168 bf16 289 us against 209).  One where two rows do not fit, 2 * columns * (sizeof X + sizeof R * (2 with
+// grad_stream, else 1)) > MAX_DYNAMIC_SMEM: float32 rows of more than 14464 columns, of more than 9642 with grad_stream, and
+// 16-bit rows with a float32 stream and grad_stream of more than 11571.
 //
 // EXACT: every thread has VPT vectors (7168 columns: 4 x 224 threads), so that no vector is predicated: with the weight kept in
 // registers, 8192 x 7168 bf16 94 -> 79 us.
@@ -293,8 +297,8 @@ k_add_rms_norm_backward(const uint8_t* grad_y, long long grad_y_pitch, const uin
   }
 }
 
-// dweight[c] = sum of the rows of `partial`, rounded once: 32 columns per CTA, 16 bytes per lane (four rows a warp and load), all of
-// a thread's loads in flight at once.
+// dweight[c] = sum of the rows of `partial`, rounded once: 32 columns per CTA, 16 bytes per lane (four rows a warp and load),
+// all of a thread's loads in flight at once.
 constexpr int WEIGHT_GRAD_WARPS = 16;
 __global__ void __launch_bounds__(WEIGHT_GRAD_WARPS * 32)
 k_norm_weight_grad(const float* partial, int rows, int columns, int type, void* grad_weight) {
@@ -345,17 +349,26 @@ k_norm_weight_grad(const float* partial, int rows, int columns, int type, void* 
 constexpr int MAX_DYNAMIC_SMEM = 227 * 1024 - 1024;   // of a CTA, less the static arrays
 
 // Vectors of eight columns per thread.  Forward: few tokens want many threads each (a CTA's latency is the call's), many tokens
-// few and fat ones (the row's sum costs per warp).  us at 7168 columns, two / four vectors: 1 token 2.3 / 2.8, 333 tokens
-// 4.2 / 5.0, 1500 tokens 11.7 / 11.8, 16384 tokens 130 / 125 (e4m3 out), 8192 tokens without a residual 46 / 40.
+// few and fat ones (the row's sum costs per warp).  us with two / four vectors:
+//   bf16, e4m3 out, 7168 columns: 1 token 2.35 / 2.89, 700 tokens 8.8 / 9.5, 8192 tokens 66.3 / 64.7, 16384 130 / 124, 8192 without
+//   a residual 46 / 40; 2048 columns: 1 token 1.9 / 2.6, 700 tokens 4.2 / 4.7.
+// The rule is one for all widths and types, and above 1024 tokens two would be faster outside of wide 16-bit rows: 1100 x
+// 7168 bf16 12.1 / 12.9, 8192 x 2048 bf16 19.5 / 20.8, 8192 x 7168 with a float32 stream 95.5 / 97.3, 1100 x 2048 float32 6.2
+// / 7.9. Another number of threads adds a row's squares in another order: see the note on batch sizes at add_rms_norm in
+// norm.py.
 static int forward_vpt(int T, int n_vec) { return n_vec > 1024 || (n_vec > 64 && T > 1024) ? 4 : n_vec > 32 ? 2 : 1; }
-// Backward: four where they leave two CTAs per SM (16-bit rows), us at 8192 x 7168 with two / four: bf16 86 / 79, bf16 with a
-// float32 stream 143 / 158; bf16 at 2048 columns 29 / 31.
+// Backward, us with two / four vectors: 8192 tokens of 7168 columns bf16 75.0 / 75.5, f16 91 / 74, bf16 with a float32 stream
+// 142 / 156, float32 151 / 163; 6144 columns f16 65.8 / 64.2; 4096 columns bf16 46.4 / 48.0; 2048 columns 25.8 / 27.6; 700
+// tokens of 7168 columns bf16 13.5 / 13.2.
 static int backward_vpt(bool wide_stream, int n_vec) {
   return n_vec > 1024 || (n_vec > 512 && !wide_stream) ? 4 : n_vec > 32 ? 2 : 1;
 }
-// Tokens that a CTA of the backward kernel works on at once.  More of them leave fewer rows of partial sums to add (us with about
-// 256 / 512 threads per CTA: 8192 x 2048 29.3 / 27.2, 4096 x 7168 45.1 / 42.2, 1000 x 4096 15.2 / 12.5), as long as the SMs are
-// evenly used (333 x 7168 8.4 / 10.3: 84 CTAs with four tokens each) and a small batch has a CTA for each token.
+// Tokens that a CTA of the backward kernel works on at once.  More of them leave fewer rows of partial sums to add (us with
+// about 256 / 512 threads per CTA: 8192 x 2048 29.3 / 27.2, 4096 x 7168 45.1 / 42.2, 1000 x 4096 15.2 / 12.5), as long as the
+// SMs are evenly used (333 x 7168 7.9 / 9.5: 84 CTAs with four tokens each) and a small batch has a CTA for each token (us
+// with one token / 512 threads per CTA: 64 x 512 3.2 / 5.0, 64 x 2048 4.2 / 4.7, 64 x 7168 6.2 / 6.3).  The limit of 64 suits
+// wide rows (200 x 4096 6.7 / 6.3, 333 x 2048 5.5 / 4.9); narrow ones would gain from one token per CTA far above it (65 x
+// 512 3.3 / 5.1, 1000 x 512 4.7 / 5.3, 2000 x 512 6.2 / 5.6).
 static int backward_groups(int T, int row_threads, int num_sms) {
   const int most = MAX_WARPS * 32 / row_threads, half = MAX_WARPS * 16 / row_threads;
   if (T <= 64) return 1;

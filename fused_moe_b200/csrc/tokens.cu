@@ -169,7 +169,8 @@ __device__ __forceinline__ TokenPairs token_pairs(const int* scatter_map, const 
   return p;
 }
 
-// CTA i's share of the rows are the `per` rows from i * per on (at most 32: rows_per_cta()), one per lane of every warp; -1: none.
+// CTA i's share of the rows are the `per` rows from i * per on (at most 32: rows_per_cta()), one per lane of every warp; -1:
+// none.
 __device__ __forceinline__ int share_row(int per, int rows) {
   const int lane = threadIdx.x & 31, row = blockIdx.x * per + lane;
   return lane < per && row < rows ? row : -1;
@@ -204,8 +205,8 @@ k_token_gather(const uint8_t* x, long long x_pitch, int T, int K, int rows, int 
   pdl_wait();
   const int t = blockIdx.x;
   const int part = (pieces + gridDim.y - 1) / gridDim.y, begin = blockIdx.y * part, end = min(begin + part, pieces);
-  // the share's two loads depend on one another: one ahead of those of the token's pairs and one behind, so that nothing waits for
-  // either (1 token 2.2 us, 64 tokens 4.2; both behind the token's work 2.3 and 4.5)
+  // the share's two loads depend on one another: one ahead of those of the token's pairs and one behind, so that nothing
+  // waits for either (1 token 2.2 us, 64 tokens 4.2; both behind the token's work 2.3 and 4.5)
   const int pair = share_pair(row_pairs, per, rows);
   TokenPairs pairs = {-1, 1.f, 0u};
   if (t < T) pairs = token_pairs(scatter_map, nullptr, t, K, rows);
